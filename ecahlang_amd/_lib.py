@@ -36,6 +36,25 @@ SIGNATURES: dict[str, tuple] = {
         [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64,
          _vp, _vp, _i32, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp],
     ),
+    "pkv_append_paged_kv_cache_fp8": (
+        _i32,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp,
+         _i32, _i32, _i32, _i32, _i32, _vp, _vp],
+    ),
+    "pkv_append_paged_kv_cache_norm_rope": (
+        _i32,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _f32, _vp, _vp, _i64,
+         _i32, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _vp,
+         _vp],
+    ),
+    "pkv_read_paged_kv_cache_fp8": (
+        _i32, [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _i32, _vp]),
+    "pkv_decode_fp8_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
+    "pkv_batch_decode_fp8": (
+        _i32,
+        [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32,
+         _f32, _i32, _vp, _i64, _vp, _i64, _i64, _i32, _vp],
+    ),
     "pkv_decode_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i64]),
     "pkv_decode_workspace_init": (_i32, [_vp, _i32, _vp]),
     "pkv_decode_schedule_layout": (_i32, [_i32, _i32, _i32, _i32, _i64, _i64, _vp]),

@@ -1,0 +1,153 @@
+// The 8-bit cache format and its row arithmetic.
+//
+// A row x[0 .. D) of one token and KV head is kept as e4m3 codes (OCP: 4 exponent bits, bias 7, 3
+// mantissa bits, largest value 448, 0x7F / 0xFF NaN) and one E8M0 scale byte e, the power of two
+// 2^(e - 127): the smallest one >= 2^-126 with max|x| <= 448 * 2^(e - 127).  A power of two, and not
+// max|x| / 448, because e4m3 rounds relative to the value, so a scale up to twice as large costs no
+// precision (only values under max|x| / 2^14 come out coarser), and then x / scale is exact: the only
+// rounding is the one to e4m3, a row read back and written again comes out the same, and every stored
+// value is exact in bfloat16.  It also takes one byte a row where fp32 takes four.  Elements that are
+// not finite are stored as NaN; the scale is that of the others.
+//
+// Scales lie beside the cache: scale of (page, slot, head) of K at
+//   k_scales[page * scale_page_stride + head * page_size + slot]
+// (V alike), one head's slots together, since attention takes one head's tokens at a time.
+#pragma once
+#include "common.h"
+
+namespace pkv {
+namespace fp8 {
+
+// Largest finite magnitude of the row so far, as bits (the order of positive floats is that of their bits).
+__device__ __forceinline__ uint32_t amax_bits(uint32_t m, float x) {
+  const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
+  const uint32_t f = u < 0x7F800000u ? u : 0u;
+  return m > f ? m : f;
+}
+// The scale byte of a row: max|x| = a * 2^E with 1 <= a < 2 needs E - 8, or E - 7 if a > 1.75
+// (448 = 1.75 * 2^8): adding 0x1FFFFF carries into the exponent exactly for mantissas over 0x600000.
+__device__ __forceinline__ int scale_byte(uint32_t amax) {
+  const int e = (int)((amax + 0x1FFFFFu) >> 23) - 8;
+  return e < 1 ? 1 : e;
+}
+// 1 / scale for a byte that scale_byte gave (1 .. 247): exact.
+__device__ __forceinline__ float inv_scale(int e) { return __uint_as_float((uint32_t)(254 - e) << 23); }
+// Any scale byte's value (0: 2^-127, 255: NaN).
+__device__ __forceinline__ float scale_f32(uint32_t e) {
+  const uint32_t b = e == 0 ? 0x00400000u : (e == 255 ? 0x7FC00000u : e << 23);
+  return __uint_as_float(b);
+}
+// Four values, |x| <= 448 or not finite, as e4m3 (to nearest, ties to even; not finite: NaN).
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+  return (uint32_t)r;
+}
+
+// 8 consecutive elements of type T: 16-byte accesses when VEC (address a multiple of 16), else one by one.
+template <typename T, bool VEC>
+struct Eight {
+  T e[8];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC) {
+      constexpr int N = sizeof(T) / 2;
+      uint4 w[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+      __builtin_memcpy(e, w, sizeof(e));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = p[j];
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (VEC) {
+      constexpr int N = sizeof(T) / 2;
+      uint4 w[N];
+      __builtin_memcpy(w, e, sizeof(e));
+#pragma unroll
+      for (int i = 0; i < N; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = e[j];
+    }
+  }
+};
+
+// Eight codes: x[0 .. 8) times inv.
+template <bool VEC>
+__device__ __forceinline__ void store8(uint8_t* p, const float (&x)[8], float inv) {
+  const uint32_t a = pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+  const uint32_t b = pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+  if constexpr (VEC) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = (uint8_t)(a >> (8 * j)), p[4 + j] = (uint8_t)(b >> (8 * j));
+  }
+}
+
+// Reduction over groups of n lanes (n = 1, 2, 4, .. 32; wave-uniform), in registers: every lane of a
+// group gets the result.  All 64 lanes must be active.
+template <typename Op>
+__device__ __forceinline__ uint32_t group_reduce(uint32_t v, int n, Op op) {
+  if (n > 1) v = op(v, wred::dpp<0xB1>(v));   // quad_perm 1 0 3 2
+  if (n > 2) v = op(v, wred::dpp<0x4E>(v));   // quad_perm 2 3 0 1
+  if (n > 4) v = op(v, wred::dpp<0x141>(v));  // row_half_mirror (each quad holds one value)
+  if (n > 8) v = op(v, wred::dpp<0x140>(v));  // row_mirror
+  if (n > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op((uint32_t)r[0], (uint32_t)r[1]);
+  }
+  return v;
+}
+__device__ __forceinline__ uint32_t group_max(uint32_t v, int n) {
+  return group_reduce(v, n, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ float group_sum(float v, int n) {
+  return __uint_as_float(group_reduce(__float_as_uint(v), n, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+
+// Lanes a row of d elements takes, 16 elements each (8 of either half), rounded up to a power of two:
+// the row kernels take head_dim % 16 == 0 up to 512.
+inline int lanes_of(int d) {
+  int n = 1;
+  while (n < d / 16) n *= 2;
+  return n;
+}
+inline bool head_dim_ok(int d) { return d > 0 && d <= 512 && d % 16 == 0; }
+
+// Where a token goes.  `slots` null: page kv_indices[kv_indptr[b] + pos / ps], slot pos % ps; else
+// slots[i] = page * ps + slot.  False for metadata outside the sequence's pages, the list or the pool.
+struct Table {
+  const int32_t *bidx, *pos, *slots, *indices, *indptr;
+  int64_t num_indices, num_pages;
+  int32_t batch, ps;
+};
+__device__ __forceinline__ bool resolve(const Table& t, int64_t i, int& page, int& slot) {
+  if (t.slots) {
+    const int sl = t.slots[i];
+    page = sl / t.ps;
+    slot = sl - page * t.ps;
+    return sl >= 0 && page < t.num_pages;
+  }
+  const int b = t.bidx[i], p = t.pos[i];
+  if (b < 0 || b >= t.batch || p < 0) return false;
+  const int base = t.indptr[b], np = t.indptr[b + 1] - base, pi = p / t.ps;
+  if (base < 0 || pi >= np || (int64_t)base + pi >= t.num_indices) return false;
+  page = t.indices[base + pi];
+  slot = p - pi * t.ps;
+  return page >= 0 && page < t.num_pages;
+}
+
+// K or V of the destination cache, and (8 bits) its scales.
+struct Dest {
+  void *k, *v;
+  uint8_t *ks, *vs;
+  int64_t page_stride, scale_stride;
+};
+
+}  // namespace fp8
+}  // namespace pkv

@@ -63,6 +63,51 @@ class CacheView:
             raise ValueError("paged_kv_cache must live on a CUDA (HIP) device")
 
 
+FP8 = torch.float8_e4m3fn
+
+
+class ScaleView:
+    """Base pointers and page stride of an 8-bit cache's scales.
+
+    An 8-bit cache (``torch.float8_e4m3fn``, same shapes as the others) goes with one power-of-two
+    scale a token and KV head, ``torch.float8_e8m0fnu`` of shape ``[pages, 2, Hkv, page_size]``
+    (``new_kv_scales``), or a ``(k_scales, v_scales)`` pair of ``[pages, Hkv, page_size]`` for a
+    ``(k_cache, v_cache)`` pair.  A stored value is code * scale."""
+
+    __slots__ = ("k_ptr", "v_ptr", "page_stride")
+
+    def __init__(self, kv_scales, cv: CacheView):
+        if cv.dtype != FP8:
+            raise ValueError(f"kv_scales go with a float8_e4m3fn cache, not {cv.dtype}")
+        if kv_scales is None:
+            raise ValueError("a float8_e4m3fn cache needs kv_scales")
+        shape = (cv.num_pages, cv.num_kv_heads, cv.page_size)
+        pair = isinstance(kv_scales, (tuple, list))
+        parts = tuple(kv_scales) if pair else (kv_scales,)
+        want = shape if pair else (shape[0], 2) + shape[1:]
+        if pair and len(parts) != 2:
+            raise ValueError("kv_scales must be one tensor or a (k_scales, v_scales) pair")
+        for t in parts:
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.float8_e8m0fnu or tuple(t.shape) != want:
+                raise ValueError(f"kv_scales must be float8_e8m0fnu {list(want)}")
+            if not t.is_contiguous():
+                raise ValueError("kv_scales must be contiguous")
+            if t.device != cv.device:
+                raise ValueError(f"kv_scales are on {t.device}, the cache on {cv.device}")
+        self.k_ptr = parts[0].data_ptr()
+        n = cv.num_kv_heads * cv.page_size
+        self.v_ptr, self.page_stride = (parts[1].data_ptr(), n) if pair else (self.k_ptr + n if self.k_ptr else 0, 2 * n)
+
+
+def new_kv_scales(paged_kv_cache: torch.Tensor) -> torch.Tensor:
+    """Scales (of ones) for an 8-bit cache ``[..., pages, 2, page_size, Hkv, D]``: ``[..., pages, 2, Hkv,
+    page_size]``, ``torch.float8_e8m0fnu``."""
+    *lead, two, ps, hkv, _ = paged_kv_cache.shape
+    if two != 2 or paged_kv_cache.dtype != FP8:
+        raise ValueError("paged_kv_cache must be float8_e4m3fn [..., pages, 2, page_size, Hkv, D]")
+    return torch.full((*lead, 2, hkv, ps), 127, dtype=torch.uint8, device=paged_kv_cache.device).view(torch.float8_e8m0fnu)
+
+
 def get_seq_lens(kv_indptr: torch.Tensor, kv_last_page_len: torch.Tensor, page_size: int) -> torch.Tensor:
     """seq_len[b] = max(indptr[b+1]-indptr[b]-1, 0) * page_size + last_page_len[b] (int32)."""
     _i32(kv_indptr, "kv_indptr")
@@ -110,15 +155,23 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor,
                           batch_indices: torch.Tensor, positions: torch.Tensor,
                           paged_kv_cache: CacheT, kv_indices: torch.Tensor, kv_indptr: torch.Tensor,
                           kv_last_page_len: torch.Tensor, kv_layout: str = "NHD",
-                          err_count: torch.Tensor | None = None) -> None:
+                          err_count: torch.Tensor | None = None, kv_scales=None) -> None:
     """Scatter ``append_key/value[i]`` into page ``kv_indices[kv_indptr[b] + pos // ps]`` slot
     ``pos % ps`` with b = batch_indices[i], pos = positions[i].  Bit-exact copy.
 
     ``kv_last_page_len`` is accepted for signature parity and, as in the reference's
     dependency, not used by the scatter.  ``err_count`` (optional int32 [1]) counts tokens
     whose metadata falls outside their sequence's pages; they are skipped.
+
+    With an 8-bit cache (``torch.float8_e4m3fn``) and its ``kv_scales`` (see ``ScaleView``) the rows, fp16,
+    bf16 or fp32, are quantised as they are written: each (token, head) row gets the smallest power of
+    two s >= 2^-126 with max|x| <= 448 s as its scale and is stored as the e4m3 values nearest to x / s.
+    Elements that are not finite are stored as NaN.  head_dim must be a multiple of 16, up to 512.
     """
     cv = CacheView(paged_kv_cache, kv_layout)
+    if cv.dtype == FP8 or kv_scales is not None:
+        return _append_fp8(append_key, append_value, cv, ScaleView(kv_scales, cv), err_count,
+                           table=(batch_indices, positions, kv_indices, kv_indptr))
     for t, n in ((append_key, "append_key"), (append_value, "append_value")):
         if t.dtype != cv.dtype:
             raise ValueError(f"{n} dtype {t.dtype} differs from the cache dtype {cv.dtype}")
@@ -147,17 +200,65 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor,
         stream_ptr(cv.device)), "append_paged_kv_cache")
 
 
+def _append_fp8(append_key, append_value, cv, sv, err_count, table=None, slots=None) -> None:
+    """The append into an 8-bit cache, by ``table`` (batch_indices, positions, kv_indices, kv_indptr) or ``slots``."""
+    nnz = append_key.shape[0]
+    _rows_fp8(append_key, append_value, cv, nnz)
+    ids = dict(zip(("batch_indices", "positions", "kv_indices", "kv_indptr"), table)) if table else {"slots": slots}
+    for n, t in ids.items():
+        if _i32(t, n).device != cv.device:
+            raise ValueError(f"{n} is on {t.device}, the cache on {cv.device}")
+    if any(t.numel() < nnz for n, t in ids.items() if not n.startswith("kv_")):
+        raise ValueError("append_key, append_value and " + (" and ".join(n for n in ids if not n.startswith("kv_")))
+                         + " disagree on nnz")
+    if table and ids["kv_indptr"].numel() < 1:
+        raise ValueError("kv_indptr must have batch+1 entries")
+    ksn, ksh = _row_strides(append_key, "append_key")
+    vsn, vsh = _row_strides(append_value, "append_value")
+    err_ptr = _i32(err_count, "err_count").data_ptr() if err_count is not None else 0
+    if nnz == 0:
+        return
+    ptr = {n: t.data_ptr() for n, t in ids.items()}
+    check(lib().pkv_append_paged_kv_cache_fp8(
+        append_key.data_ptr(), ksn, ksh, append_value.data_ptr(), vsn, vsh, ptr.get("batch_indices", 0),
+        ptr.get("positions", 0), ptr.get("slots", 0), nnz, cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages,
+        sv.k_ptr, sv.v_ptr, sv.page_stride, ptr.get("kv_indices", 0),
+        ids["kv_indices"].numel() if table else 0, ptr.get("kv_indptr", 0),
+        ids["kv_indptr"].numel() - 1 if table else 0, cv.num_kv_heads, cv.head_dim, cv.page_size,
+        dtype_code(append_key.dtype), err_ptr, stream_ptr(cv.device)), "append_paged_kv_cache (8-bit cache)")
+
+
+def _rows_fp8(append_key, append_value, cv, nnz) -> None:
+    """Checks of the rows that go into an 8-bit cache."""
+    if append_key.dtype not in (torch.float16, torch.bfloat16, torch.float32) or append_value.dtype != append_key.dtype:
+        raise ValueError("append_key and append_value must share one of float16, bfloat16 and float32")
+    for t, n in ((append_key, "append_key"), (append_value, "append_value")):
+        if tuple(t.shape) != (nnz, cv.num_kv_heads, cv.head_dim):
+            raise ValueError(f"{n} must be [{nnz}, {cv.num_kv_heads}, {cv.head_dim}]")
+        if t.device != cv.device:
+            raise ValueError(f"{n} is on {t.device}, the cache on {cv.device}")
+    _head_dim_16(cv)
+
+
+def _head_dim_16(cv) -> None:
+    if cv.head_dim % 16 or not 0 < cv.head_dim <= 512:
+        raise ValueError("head_dim must be a multiple of 16, up to 512")
+
+
 def append_paged_kv_cache_slots(append_key: torch.Tensor, append_value: torch.Tensor, slots: torch.Tensor,
                                 paged_kv_cache: CacheT, kv_layout: str = "NHD",
-                                err_count: torch.Tensor | None = None) -> None:
+                                err_count: torch.Tensor | None = None, kv_scales=None) -> None:
     """``append_paged_kv_cache`` with each token's destination resolved beforehand: token i goes
     to page ``slots[i] // ps``, slot ``slots[i] % ps`` (``slots`` as the page-table gather of
     ``AutoKVCacheManager.fill_cuda_graph_metadata`` writes them).  One lookup per token instead
     of the three dependent ones through batch_indices / positions, kv_indptr and kv_indices;
     the bytes written are the same.  Tokens with a negative or out-of-pool slot are skipped and
-    counted in ``err_count``.
+    counted in ``err_count``.  With an 8-bit cache and its ``kv_scales`` the rows are quantised as
+    ``append_paged_kv_cache`` does it.
     """
     cv = CacheView(paged_kv_cache, kv_layout)
+    if cv.dtype == FP8 or kv_scales is not None:
+        return _append_fp8(append_key, append_value, cv, ScaleView(kv_scales, cv), err_count, slots=slots)
     for t, n in ((append_key, "append_key"), (append_value, "append_value")):
         if t.dtype != cv.dtype:
             raise ValueError(f"{n} dtype {t.dtype} differs from the cache dtype {cv.dtype}")
@@ -245,3 +346,116 @@ def append_paged_kv_cache_with_rope(q: torch.Tensor, append_key: torch.Tensor, a
         kv_indptr.numel() - 1, cv.num_kv_heads, cv.head_dim, cv.page_size, dtype_code(cv.dtype), err_ptr,
         stream_ptr(cv.device)), "append_paged_kv_cache_with_rope")
     return q_out
+
+
+def append_paged_kv_cache_with_norm_rope(q: torch.Tensor, append_key: torch.Tensor, append_value: torch.Tensor,
+                                         q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                                         cos: torch.Tensor, sin: torch.Tensor, batch_indices: torch.Tensor,
+                                         positions: torch.Tensor, paged_kv_cache: CacheT,
+                                         kv_indices: torch.Tensor, kv_indptr: torch.Tensor,
+                                         kv_last_page_len: torch.Tensor, kv_layout: str = "NHD", eps: float = 1e-6,
+                                         q_out: torch.Tensor | None = None, err_count: torch.Tensor | None = None,
+                                         kv_scales=None) -> torch.Tensor:
+    """RMS norm of every query and key head, rotary embedding and append, in one launch: what a model with
+    per-head query / key norms does between its projections and the attention.
+
+    ``y = x / sqrt(mean(x^2) + eps) * weight`` over the head_dim of each row of ``q`` and ``append_key``, then
+    ``y * cos + rotate_half(y) * sin``, all in fp32 and rounded once: the queries into ``q_out`` (default: a new
+    tensor; pass ``q`` to work in place), which is returned, the keys into their pages.  Values are appended
+    unchanged.  ``q_weight`` / ``k_weight`` ``[head_dim]`` (``None``: rows of that kind are rotated only; both of
+    one type) and ``cos`` / ``sin`` ``[nnz, head_dim]`` are in the rows' type or fp32; a weight that a model
+    keeps as an offset from one is passed as ``1 + w``.  The cache is in the rows' type, or an 8-bit one with
+    its ``kv_scales``: then keys (from fp32) and values are quantised as ``append_paged_kv_cache`` does it.
+    head_dim must be a multiple of 16, up to 512.  Tokens with bad metadata are skipped, but for their
+    queries, and counted in ``err_count``.
+    """
+    cv = CacheView(paged_kv_cache, kv_layout)
+    sv = ScaleView(kv_scales, cv) if cv.dtype == FP8 or kv_scales is not None else None
+    nnz, d, dt = append_key.shape[0], cv.head_dim, append_key.dtype
+    _rows_fp8(append_key, append_value, cv, nnz)
+    if sv is None and dt != cv.dtype:
+        raise ValueError(f"append_key dtype {dt} differs from the cache dtype {cv.dtype}")
+    if q.dtype != dt or q.dim() != 3 or q.shape[0] != nnz or q.shape[2] != d:
+        raise ValueError(f"q must be [{nnz}, Hq, {d}] in {dt}")
+    for a, b, shape, names in ((q_weight, k_weight, (d,), ("q_weight", "k_weight")), (cos, sin, (nnz, d), ("cos", "sin"))):
+        for t, n in zip((a, b), names):
+            if t is None and shape == (d,):
+                continue
+            if not isinstance(t, torch.Tensor) or t.dtype not in (dt, torch.float32) or tuple(t.shape) != shape or \
+                    (t.numel() and t.stride(-1) != 1):
+                raise ValueError(f"{n} must be {list(shape)} in {dt} or float32 with a unit inner stride")
+        if a is not None and b is not None and a.dtype != b.dtype:
+            raise ValueError(f"{names[0]} and {names[1]} must share one dtype")
+    if cos.stride(0) != sin.stride(0):
+        raise ValueError("cos and sin must share a row stride")
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    _i32(batch_indices, "batch_indices")
+    _i32(positions, "positions")
+    _i32(kv_indices, "kv_indices")
+    _i32(kv_indptr, "kv_indptr")
+    if batch_indices.numel() < nnz or positions.numel() < nnz:
+        raise ValueError("q, append_key, append_value, batch_indices and positions disagree on nnz")
+    if kv_indptr.numel() < 1:
+        raise ValueError("kv_indptr must have batch+1 entries")
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif q_out.shape != q.shape or q_out.dtype != q.dtype:
+        raise ValueError("q_out must match q's shape and dtype")
+    qsn, qsh = _row_strides(q, "q")
+    osn, osh = _row_strides(q_out, "q_out")
+    ksn, ksh = _row_strides(append_key, "append_key")
+    vsn, vsh = _row_strides(append_value, "append_value")
+    for t, n in ((q, "q"), (q_out, "q_out"), (q_weight, "q_weight"), (k_weight, "k_weight"), (cos, "cos"), (sin, "sin"),
+                 (batch_indices, "batch_indices"), (positions, "positions"), (kv_indices, "kv_indices"),
+                 (kv_indptr, "kv_indptr")):
+        if t is not None and t.device != cv.device:
+            raise ValueError(f"{n} is on {t.device}, the cache on {cv.device}")
+    err_ptr = _i32(err_count, "err_count").data_ptr() if err_count is not None else 0
+    if nnz == 0:
+        return q_out
+    w = q_weight if q_weight is not None else k_weight
+    check(lib().pkv_append_paged_kv_cache_norm_rope(
+        q.data_ptr(), qsn, qsh, q_out.data_ptr(), osn, osh, q.shape[1], append_key.data_ptr(), ksn, ksh,
+        append_value.data_ptr(), vsn, vsh, q_weight.data_ptr() if q_weight is not None else 0,
+        k_weight.data_ptr() if k_weight is not None else 0, dtype_code(w.dtype if w is not None else dt), float(eps),
+        cos.data_ptr(), sin.data_ptr(), cos.stride(0), dtype_code(cos.dtype), batch_indices.data_ptr(),
+        positions.data_ptr(), nnz, cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages, sv.k_ptr if sv else 0,
+        sv.v_ptr if sv else 0, sv.page_stride if sv else 0, kv_indices.data_ptr(), kv_indices.numel(),
+        kv_indptr.data_ptr(), kv_indptr.numel() - 1, cv.num_kv_heads, d, cv.page_size, dtype_code(dt), err_ptr,
+        stream_ptr(cv.device)), "append_paged_kv_cache_with_norm_rope")
+    return q_out
+
+
+def read_paged_kv_cache(paged_kv_cache: CacheT, kv_scales, kv_indices: torch.Tensor, kv_indptr: torch.Tensor,
+                        dtype: torch.dtype, out: torch.Tensor | None = None, kv_layout: str = "NHD") -> torch.Tensor:
+    """An 8-bit cache's listed pages in fp16, bf16 or fp32: page i of the result ``[len(kv_indices), 2,
+    page_size, Hkv, D]`` holds the values of page ``kv_indices[i]``, for i < ``kv_indptr[-1]``, so with the
+    page ids 0, 1, 2, ... it stands for the cache wherever one of ``dtype`` is read (the prefill wrapper does
+    this by itself).  bf16 and fp32 hold every value exactly, fp16 those in its range.  Whole pages are
+    read, with the slots past a sequence's end; an id outside the pool gives zeros; pages of ``out`` past
+    the list are left as they were.  head_dim must be a multiple of 16, up to 512.
+    """
+    cv = CacheView(paged_kv_cache, kv_layout)
+    sv = ScaleView(kv_scales, cv)
+    _head_dim_16(cv)
+    _i32(kv_indices, "kv_indices")
+    _i32(kv_indptr, "kv_indptr")
+    if kv_indptr.numel() < 1:
+        raise ValueError("kv_indptr must have batch+1 entries")
+    if kv_indices.device != cv.device or kv_indptr.device != cv.device:
+        raise ValueError("kv_indices and kv_indptr must be on the cache's device")
+    code = dtype_code(dtype)
+    n = kv_indices.numel()
+    shape = (n, 2, cv.page_size, cv.num_kv_heads, cv.head_dim)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=cv.device)
+    elif tuple(out.shape) != shape or out.dtype != dtype or not out.is_contiguous() or out.device != cv.device:
+        raise ValueError(f"out must be {list(shape)} in {dtype}, contiguous, on the cache's device")
+    if n == 0 or kv_indptr.numel() == 1:
+        return out
+    check(lib().pkv_read_paged_kv_cache_fp8(
+        cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages, sv.k_ptr, sv.v_ptr, sv.page_stride, kv_indices.data_ptr(),
+        n, kv_indptr.data_ptr(), kv_indptr.numel() - 1, cv.num_kv_heads, cv.head_dim, cv.page_size, out.data_ptr(),
+        code, stream_ptr(cv.device)), "read_paged_kv_cache")
+    return out

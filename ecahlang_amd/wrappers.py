@@ -25,9 +25,9 @@ import numpy as np
 import torch
 
 from ._lib import check, dtype_code, lib, stream_ptr
-from .ops import CacheView, _i32
+from .ops import FP8, CacheView, ScaleView, _i32, read_paged_kv_cache
 
-_STR_DTYPES = {"float16": torch.float16, "half": torch.float16, "bfloat16": torch.bfloat16,
+_STR_DTYPES = {"float8_e4m3fn": FP8, "float16": torch.float16, "half": torch.float16, "bfloat16": torch.bfloat16,
                "float32": torch.float32, "float": torch.float32}
 
 
@@ -148,10 +148,13 @@ class BatchDecodeWithPagedKVCacheWrapper:
             q_data_type = data_type
         self._q_dtype = _as_dtype(q_data_type)
         self._kv_dtype = _as_dtype(kv_data_type) if kv_data_type is not None else self._q_dtype
-        if self._kv_dtype != self._q_dtype:
-            raise NotImplementedError("q and kv must share one dtype")
+        self._fp8 = self._kv_dtype == FP8 and self._q_dtype in (torch.float16, torch.bfloat16)
+        if self._kv_dtype != self._q_dtype and not self._fp8:
+            raise NotImplementedError("q and kv must share one dtype, or be float16 / bfloat16 and float8_e4m3fn")
         self._sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(self._d)
         dev = indptr.device
+        if self._fp8:
+            return self._plan_fp8(dev, num_ctas)
         self._mfma = bool(lib().pkv_decode_uses_mfma(dtype_code(self._q_dtype), self._d, self._hq,
                                                      self._hkv, self._batch)) and self._ps == 16
         env = os.environ.get("PKV_DECODE_CTAS")
@@ -204,13 +207,51 @@ class BatchDecodeWithPagedKVCacheWrapper:
             self._flags |= _DECODE_PLANNED
         self._planned = True
 
+    def _plan_fp8(self, dev: torch.device, num_ctas: int | None) -> None:
+        """An 8-bit cache's decode needs no schedule (it reads the page table when it runs): room for its
+        partials, and zeroed counters, one a sequence and block of 16 query heads of a KV head."""
+        if self._d not in (64, 128, 256):
+            raise ValueError("head_dim must be 64, 128 or 256 for a float8_e4m3fn cache")
+        if self._batch < 1 or self._ps < 1:
+            raise ValueError("an empty batch or page size cannot be planned")
+        self._mfma, self._flags = False, 0
+        self._ctas = int(num_ctas) if num_ctas is not None else 2 * _num_cus(dev)
+        if self._ctas <= 0:
+            raise ValueError("num_ctas must be positive")
+        ws = self._workspace
+        need = lib().pkv_decode_fp8_workspace_bytes(self._batch, self._hq, self._hkv, self._d, self._ctas)
+        if need < 0:
+            check(int(need), "decode plan")
+        if need > ws.numel() * ws.element_size():
+            raise RuntimeError(f"decode workspace too small: need {need} bytes")
+        counters = self._batch * self._hkv * -(-self._hq // self._hkv // 16)
+        if counters > self._counters_ready:
+            check(lib().pkv_decode_workspace_init(ws.data_ptr(), counters, stream_ptr(dev)), "decode plan")
+        self._counters_ready = counters  # (the words after these are overwritten)
+        self._planned = True
+
+    def _run_fp8(self, q: torch.Tensor, cv: CacheView, kv_scales, out: torch.Tensor) -> torch.Tensor:
+        sv = ScaleView(kv_scales, cv)
+        if (q.data_ptr() | q.stride(0) * 2 | q.stride(1) * 2) % 16:  # (rows are read 16 bytes at a time)
+            q = q.clone(memory_format=torch.contiguous_format)
+        check(lib().pkv_batch_decode_fp8(
+            q.data_ptr(), q.stride(0), q.stride(1), cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages, sv.k_ptr, sv.v_ptr,
+            sv.page_stride, self._indptr.data_ptr(), self._indices.data_ptr(), self._indices.numel(),
+            self._last.data_ptr(), self._batch, self._hq, self._hkv, self._d, self._ps, self._sm_scale, self._ctas,
+            self._workspace.data_ptr(), self._workspace.numel() * self._workspace.element_size(), out.data_ptr(),
+            out.stride(0), out.stride(1), dtype_code(q.dtype), stream_ptr(q.device)),
+            "BatchDecodeWithPagedKVCacheWrapper.run")
+        return out
+
     def run(self, q: torch.Tensor, paged_kv_cache, *args, q_scale=None, k_scale=None,
             v_scale=None, out: torch.Tensor | None = None, lse=None, return_lse: bool = False,
-            window_left=None, enable_pdl=None, force_valu: bool = False, append_kv=None) -> torch.Tensor:
+            window_left=None, enable_pdl=None, force_valu: bool = False, append_kv=None,
+            kv_scales=None) -> torch.Tensor:
         """FlashInfer's run (ecahlang/main.py:68).  Extension: ``append_kv=(k, v)``, each
         [batch, num_kv_heads, head_dim] with unit inner stride, first appends token b's rows at
         position seq_len_b - 1 (the decode step's append through the CUDA-graph metadata,
-        ecahlang/manager.py:270-280) -- in the same launch on the matrix-core path."""
+        ecahlang/manager.py:270-280) -- in the same launch on the matrix-core path.  ``kv_scales``: the
+        scales of a float8_e4m3fn cache (``ops.ScaleView``)."""
         if not self._planned:
             raise RuntimeError("plan() must be called before run()")
         if torch.cuda.is_current_stream_capturing():
@@ -222,14 +263,20 @@ class BatchDecodeWithPagedKVCacheWrapper:
         cv = CacheView(paged_kv_cache, self._kv_layout)
         if q.dim() != 3 or q.shape != (self._batch, self._hq, self._d) or q.stride(2) != 1:
             raise ValueError(f"q must be [{self._batch}, {self._hq}, {self._d}] with unit inner stride")
-        if q.dtype != self._q_dtype or cv.dtype != self._q_dtype:
-            raise ValueError(f"q / cache dtype must be {self._q_dtype}")
+        if q.dtype != self._q_dtype or cv.dtype != self._kv_dtype:
+            raise ValueError(f"q dtype must be {self._q_dtype}, cache dtype {self._kv_dtype}")
         if (cv.num_kv_heads, cv.head_dim, cv.page_size) != (self._hkv, self._d, self._ps):
             raise ValueError("cache geometry differs from plan()")
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
             raise ValueError("out must match q's shape and dtype")
+        if self._fp8:
+            if append_kv is not None or force_valu:
+                raise NotImplementedError("append_kv and force_valu are not implemented for float8_e4m3fn caches")
+            return self._run_fp8(q, cv, kv_scales, out)
+        if kv_scales is not None:
+            raise ValueError("kv_scales go with a float8_e4m3fn cache")
         if append_kv is not None:
             k, v = append_kv
             for t, n in ((k, "k"), (v, "v")):
@@ -316,7 +363,10 @@ class BatchPrefillWithPagedKVCacheWrapper:
 
     With a 16-bit cache and a power-of-two group, ``plan`` keeps its work list in the workspace and
     a run its partials: the buffer belongs to one such wrapper, and its runs follow its plan on one
-    stream or streams ordered after each other.  All other shapes leave the workspace alone."""
+    stream or streams ordered after each other.  All other shapes leave the workspace alone.
+
+    Over a float8_e4m3fn cache (``kv_data_type``; float16 / bfloat16 queries) a run first reads the planned pages
+    back to the queries' type (``ops.read_paged_kv_cache``), into memory of its own, and attends those."""
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD",
                  use_cuda_graph: bool = False, qo_indptr_buf=None, paged_kv_indptr_buf=None,
@@ -360,8 +410,9 @@ class BatchPrefillWithPagedKVCacheWrapper:
         self._causal = bool(causal)
         self._q_dtype = _as_dtype(q_data_type)
         self._kv_dtype = _as_dtype(kv_data_type) if kv_data_type is not None else self._q_dtype
-        if self._kv_dtype != self._q_dtype:
-            raise NotImplementedError("q and kv must share one dtype")
+        self._fp8 = self._kv_dtype == FP8 and self._q_dtype in (torch.float16, torch.bfloat16)
+        if self._kv_dtype != self._q_dtype and not self._fp8:
+            raise NotImplementedError("q and kv must share one dtype, or be float16 / bfloat16 and float8_e4m3fn")
         self._sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(self._d)
         self._mfma = bool(lib().pkv_prefill_mfma_supported(dtype_code(self._q_dtype), self._d, self._hq,
                                                           self._hkv, self._ps))
@@ -377,7 +428,18 @@ class BatchPrefillWithPagedKVCacheWrapper:
             self._mfma = self._batch > 0 and self._sm_scale > 0 and not torch.cuda.is_current_stream_capturing()
         if self._mfma:
             self._schedule(qo_indptr.device)
+        if self._fp8:
+            self._plan_read()
         self._planned = True
+
+    def _plan_read(self) -> None:
+        """The pages that a run reads back (the listed ones; while capturing, as many as the list can hold), and
+        their numbers there: 0, 1, 2, ..."""
+        n = self._indices.numel()
+        if self._batch and not torch.cuda.is_current_stream_capturing():
+            n = min(n, max(0, self._n_pages if self._mfma else int(self._indptr[-1])))
+        self._read_list = self._indices[:n]
+        self._indices = torch.arange(n, dtype=torch.int32, device=self._indptr.device)
 
     # rows per matrix-core work item (8 waves x 32 rows, fp32 8 x 16): rows / g query tokens of one KV head
     _ROWS, _ROWS_F32 = 256, 128
@@ -390,7 +452,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         n = self._batch + 1
         table = torch.cat((self._qo_indptr, self._indptr, self._last)).cpu().numpy()
         qo, kp, last = table[:n], table[n:2 * n], table[2 * n:]
-        self._nnz_q = int(qo[-1])
+        self._nnz_q, self._n_pages = int(qo[-1]), int(kp[-1])
         ws = self._workspace
         ws_bytes = ws.numel() * ws.element_size() if isinstance(ws, torch.Tensor) else 0
         g = self._hq // self._hkv
@@ -445,7 +507,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
 
     def run(self, q: torch.Tensor, paged_kv_cache, *args, q_scale=None, k_scale=None,
             v_scale=None, out: torch.Tensor | None = None, lse=None, return_lse: bool = False,
-            enable_pdl=None, window_left=None, force_valu: bool = False) -> torch.Tensor:
+            enable_pdl=None, window_left=None, force_valu: bool = False, kv_scales=None) -> torch.Tensor:
         if not self._planned:
             raise RuntimeError("plan() must be called before run()")
         if return_lse or lse is not None:
@@ -453,8 +515,10 @@ class BatchPrefillWithPagedKVCacheWrapper:
         cv = CacheView(paged_kv_cache, self._kv_layout)
         if q.dim() != 3 or q.shape[1:] != (self._hq, self._d) or q.stride(2) != 1:
             raise ValueError(f"q must be [nnz, {self._hq}, {self._d}] with unit inner stride")
-        if q.dtype != self._q_dtype or cv.dtype != self._q_dtype:
-            raise ValueError(f"q / cache dtype must be {self._q_dtype}")
+        if q.dtype != self._q_dtype or cv.dtype != self._kv_dtype:
+            raise ValueError(f"q dtype must be {self._q_dtype}, cache dtype {self._kv_dtype}")
+        if kv_scales is not None and not self._fp8:
+            raise ValueError("kv_scales go with a float8_e4m3fn cache")
         if (cv.num_kv_heads, cv.head_dim, cv.page_size) != (self._hkv, self._d, self._ps):
             raise ValueError("cache geometry differs from plan()")
         nnz = q.shape[0]
@@ -462,6 +526,10 @@ class BatchPrefillWithPagedKVCacheWrapper:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
             raise ValueError("out must match q's shape and dtype")
+        if self._fp8:
+            pages = read_paged_kv_cache(paged_kv_cache, kv_scales, self._read_list, self._indptr, self._q_dtype,
+                                        kv_layout=self._kv_layout)
+            cv = CacheView(pages)
         aligned = q.data_ptr() % 16 == 0 and (q.stride(0) * q.element_size()) % 16 == 0 and \
             (q.stride(1) * q.element_size()) % 16 == 0
         mfma = self._mfma and aligned and not force_valu

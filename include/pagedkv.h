@@ -102,6 +102,76 @@ int pkv_append_paged_kv_cache_rope(const void* q, int64_t q_stride_n, int64_t q_
                                    int32_t batch, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
                                    int32_t dtype, int32_t* err_count, void* stream);
 
+/* ---- 8-bit caches
+ *
+ * Codes are OCP e4m3 (1 byte, addressed like the other caches' elements, with page_stride in bytes);
+ * each (token, KV head) row x of K and of V has one E8M0 scale byte e: the row's values are code *
+ * 2^(e - 127).  Scale of (page, head, slot) of K: k_scales[page * scale_page_stride + head * page_size
+ * + slot], V alike (for one tensor [pages, 2, Hkv, page_size]: v_scales = k_scales + Hkv * page_size,
+ * scale_page_stride = 2 * Hkv * page_size).  The writers choose the smallest power of two >= 2^-126
+ * with max|x| <= 448 * scale over the row's finite elements (e = 1 .. 247) and store the e4m3 value
+ * nearest to x / scale, ties to even; an element that is not finite becomes NaN.  head_dim is a
+ * multiple of 16, up to 512 (the decode: 64, 128 or 256). */
+
+/* pkv_append_paged_kv_cache (slots NULL) or pkv_append_paged_kv_cache_slots (slots given:
+ * batch_indices, positions, kv_indices and kv_indptr are not read) into an 8-bit cache.  `dtype` is
+ * the rows' type (fp16, bf16 or fp32).  Tokens with bad metadata are skipped and counted in
+ * *err_count (may be NULL) once per token, K / V and head. */
+int pkv_append_paged_kv_cache_fp8(const void* append_key, int64_t k_stride_n, int64_t k_stride_h,
+                                  const void* append_value, int64_t v_stride_n, int64_t v_stride_h,
+                                  const int32_t* batch_indices, const int32_t* positions, const int32_t* slots,
+                                  int32_t nnz, void* k_cache, void* v_cache, int64_t page_stride,
+                                  int64_t num_pages, void* k_scales, void* v_scales, int64_t scale_page_stride,
+                                  const int32_t* kv_indices, int64_t num_indices, const int32_t* kv_indptr,
+                                  int32_t batch, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                                  int32_t dtype, int32_t* err_count, void* stream);
+
+/* RMS norm of every query and key head, the rotary embedding and the append in one launch (models
+ * that normalise their heads run q_norm / k_norm and apply_rotary_pos_emb just before the hook's
+ * append, ecahlang/main.py:62-66).  A query or key row x: y = x / sqrt(mean(x^2) + eps) * weight,
+ * then y * cos + rotate_half(y) * sin; fp32 throughout, rounded once.  q_weight / k_weight [head_dim]
+ * (NULL: rows of that kind are rotated only) have type weight_dtype, cos / sin [nnz, head_dim] type
+ * cs_dtype: `dtype` or fp32.  With k_scales / v_scales the cache is an 8-bit one, else (both NULL)
+ * of type `dtype`; value rows are rounded to e4m3, or copied.  q_out == q works in place.  Bad
+ * metadata is skipped and counted once per token in *err_count (may be NULL); the token's query
+ * rows are written all the same. */
+int pkv_append_paged_kv_cache_norm_rope(
+    const void* q, int64_t q_stride_n, int64_t q_stride_h, void* q_out, int64_t qo_stride_n, int64_t qo_stride_h,
+    int32_t num_qo_heads, const void* append_key, int64_t k_stride_n, int64_t k_stride_h, const void* append_value,
+    int64_t v_stride_n, int64_t v_stride_h, const void* q_weight, const void* k_weight, int32_t weight_dtype,
+    float eps, const void* cos, const void* sin, int64_t cs_stride_n, int32_t cs_dtype,
+    const int32_t* batch_indices, const int32_t* positions, int32_t nnz, void* k_cache, void* v_cache,
+    int64_t page_stride, int64_t num_pages, void* k_scales, void* v_scales, int64_t scale_page_stride,
+    const int32_t* kv_indices, int64_t num_indices, const int32_t* kv_indptr, int32_t batch, int32_t num_kv_heads,
+    int32_t head_dim, int32_t page_size, int32_t dtype, int32_t* err_count, void* stream);
+
+/* Listed page i (kv_indices[i], i < min(kv_indptr[batch], num_indices)) of an 8-bit cache as page i
+ * of out [num_indices, 2, page_size, Hkv, head_dim] in fp16, bf16 or fp32: what the prefill kernels
+ * read, with kv_indices 0, 1, 2, ...  Whole pages, the slots past a sequence's end among them; an id
+ * outside the pool gives zeros; out pages past the list are left as they were. */
+int pkv_read_paged_kv_cache_fp8(const void* k_cache, const void* v_cache, int64_t page_stride, int64_t num_pages,
+                                const void* k_scales, const void* v_scales, int64_t scale_page_stride,
+                                const int32_t* kv_indices, int64_t num_indices, const int32_t* kv_indptr,
+                                int32_t batch, int32_t num_kv_heads, int32_t head_dim, int32_t page_size, void* out,
+                                int32_t dtype, void* stream);
+
+/* Decode attention over an 8-bit cache: pkv_batch_decode's contract with fp16 or bf16 queries (`dtype`),
+ * head_dim 64, 128 or 256, any page size and group.  No plan: the page table is read when the call
+ * runs.  The workspace (pkv_decode_fp8_workspace_bytes) starts with batch * Hkv * ceil(group / 16)
+ * arrival counters, zeroed once (pkv_decode_workspace_init of that many) and left at zero; it
+ * belongs to one call at a time.  q rows, the caches and page_stride have to be multiples of 16
+ * bytes, for a page_size that is a multiple of 16 the scales and their stride of 4. */
+int64_t pkv_decode_fp8_workspace_bytes(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+                                       int32_t head_dim, int32_t num_ctas);
+int pkv_batch_decode_fp8(const void* q, int64_t q_stride_n, int64_t q_stride_h, const void* k_cache,
+                         const void* v_cache, int64_t page_stride, int64_t num_pages, const void* k_scales,
+                         const void* v_scales, int64_t scale_page_stride, const int32_t* kv_indptr,
+                         const int32_t* kv_indices, int64_t num_indices, const int32_t* kv_last_page_len,
+                         int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+                         int32_t page_size, float sm_scale, int32_t num_ctas, void* workspace,
+                         int64_t workspace_bytes, void* out, int64_t o_stride_n, int64_t o_stride_h,
+                         int32_t dtype, void* stream);
+
 /* Smallest workspace pkv_decode_plan and pkv_batch_decode need for this geometry (num_indices =
  * length of the kv_indices buffer): the host half of BatchDecodeWithPagedKVCacheWrapper.plan
  * (ecahlang/main.py:341-347, :444-455).  The reference hands the wrapper a 128 MiB buffer
