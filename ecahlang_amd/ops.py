@@ -10,7 +10,8 @@ from typing import Tuple, Union
 
 import torch
 
-from ._lib import check, dtype_code, lib, stream_ptr
+from ._lib import (CALL_APPEND_FP8, CALL_NORM_ROPE, CALL_READ_FP8, DTYPE_CODE, call, check, dtype_code, lib,
+                   stream_ptr)
 
 CacheT = Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]
 
@@ -35,7 +36,7 @@ class CacheView:
                  "head_dim", "dtype", "device")
 
     def __init__(self, paged_kv_cache: CacheT, kv_layout: str = "NHD"):
-        if kv_layout.upper() != "NHD":
+        if kv_layout != "NHD" and kv_layout.upper() != "NHD":
             raise NotImplementedError("only the NHD cache layout is implemented (the reference uses NHD)")
         if isinstance(paged_kv_cache, (tuple, list)):
             k, v = paged_kv_cache
@@ -47,19 +48,20 @@ class CacheView:
             self.k_ptr, self.v_ptr = k.data_ptr(), v.data_ptr()
             self.num_pages, self.page_size, self.num_kv_heads, self.head_dim = k.shape
             self.page_stride = k.stride(0)
-            self.dtype, self.device = k.dtype, k.device
         else:
-            c = paged_kv_cache
-            if c.dim() != 5 or c.shape[1] != 2:
+            k = paged_kv_cache
+            shape = k.shape
+            if len(shape) != 5 or shape[1] != 2:
                 raise ValueError("paged_kv_cache must be [pages, 2, page_size, Hkv, D] (NHD)")
-            if not c.is_contiguous():
+            if not k.is_contiguous():
                 raise ValueError("paged_kv_cache must be contiguous")
-            self.num_pages, _, self.page_size, self.num_kv_heads, self.head_dim = c.shape
-            self.k_ptr = c.data_ptr()
-            self.v_ptr = self.k_ptr + c.stride(1) * c.element_size() if self.k_ptr else 0
-            self.page_stride = c.stride(0)
-            self.dtype, self.device = c.dtype, c.device
-        if not (self.device.type == "cuda"):
+            self.num_pages, _, self.page_size, self.num_kv_heads, self.head_dim = shape
+            self.k_ptr = p = k.data_ptr()
+            half = shape[2] * shape[3] * shape[4]
+            self.v_ptr = p + half * k.element_size() if p else 0
+            self.page_stride = 2 * half
+        self.dtype, self.device = k.dtype, k.device
+        if not k.is_cuda:
             raise ValueError("paged_kv_cache must live on a CUDA (HIP) device")
 
 
@@ -81,22 +83,24 @@ class ScaleView:
             raise ValueError(f"kv_scales go with a float8_e4m3fn cache, not {cv.dtype}")
         if kv_scales is None:
             raise ValueError("a float8_e4m3fn cache needs kv_scales")
-        shape = (cv.num_pages, cv.num_kv_heads, cv.page_size)
+        pages, ps, hkv = cv.num_pages, cv.page_size, cv.num_kv_heads
         pair = isinstance(kv_scales, (tuple, list))
-        parts = tuple(kv_scales) if pair else (kv_scales,)
-        want = shape if pair else (shape[0], 2) + shape[1:]
-        if pair and len(parts) != 2:
+        if pair and len(kv_scales) != 2:
             raise ValueError("kv_scales must be one tensor or a (k_scales, v_scales) pair")
-        for t in parts:
-            if not isinstance(t, torch.Tensor) or t.dtype != torch.float8_e8m0fnu or tuple(t.shape) != want:
+        want = (pages, hkv, ps) if pair else (pages, 2, hkv, ps)
+        for t in kv_scales if pair else (kv_scales,):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.float8_e8m0fnu or t.shape != want:
                 raise ValueError(f"kv_scales must be float8_e8m0fnu {list(want)}")
             if not t.is_contiguous():
                 raise ValueError("kv_scales must be contiguous")
             if t.device != cv.device:
                 raise ValueError(f"kv_scales are on {t.device}, the cache on {cv.device}")
-        self.k_ptr = parts[0].data_ptr()
-        n = cv.num_kv_heads * cv.page_size
-        self.v_ptr, self.page_stride = (parts[1].data_ptr(), n) if pair else (self.k_ptr + n if self.k_ptr else 0, 2 * n)
+        n = hkv * ps
+        if pair:
+            self.k_ptr, self.v_ptr, self.page_stride = kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), n
+        else:
+            self.k_ptr = p = kv_scales.data_ptr()
+            self.v_ptr, self.page_stride = p + n if p else 0, 2 * n
 
 
 def new_kv_scales(paged_kv_cache: torch.Tensor) -> torch.Tensor:
@@ -170,8 +174,8 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor,
     """
     cv = CacheView(paged_kv_cache, kv_layout)
     if cv.dtype == FP8 or kv_scales is not None:
-        return _append_fp8(append_key, append_value, cv, ScaleView(kv_scales, cv), err_count,
-                           table=(batch_indices, positions, kv_indices, kv_indptr))
+        return _append_fp8(append_key, append_value, cv, ScaleView(kv_scales, cv), err_count, batch_indices, positions,
+                           kv_indices, kv_indptr)
     for t, n in ((append_key, "append_key"), (append_value, "append_value")):
         if t.dtype != cv.dtype:
             raise ValueError(f"{n} dtype {t.dtype} differs from the cache dtype {cv.dtype}")
@@ -200,49 +204,68 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor,
         stream_ptr(cv.device)), "append_paged_kv_cache")
 
 
-def _append_fp8(append_key, append_value, cv, sv, err_count, table=None, slots=None) -> None:
-    """The append into an 8-bit cache, by ``table`` (batch_indices, positions, kv_indices, kv_indptr) or ``slots``."""
+def _ids(t: torch.Tensor, name: str, dev: torch.device) -> int:
+    """Address of an int32 index tensor on the cache's device."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or not t.is_contiguous():
+        _i32(t, name)
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, name: str, shape: tuple, dt: torch.dtype, dev: torch.device) -> tuple:
+    """Strides of [n, heads, head_dim] rows, whose type, shape and place are checked."""
+    if t.dtype != dt:
+        raise ValueError(f"{name} must be {dt}, not {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}")
+    st = t.stride()
+    if st[2] != 1:
+        raise ValueError(f"{name} must have a unit inner stride")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
+    return st
+
+
+_ROW_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def _row_dtype(t: torch.Tensor, cv: CacheView) -> torch.dtype:
+    dt = t.dtype
+    if dt not in _ROW_DTYPES:
+        raise ValueError(f"rows must be float16, bfloat16 or float32, not {dt}")
+    if cv.head_dim % 16 or not 0 < cv.head_dim <= 512:
+        raise ValueError("head_dim must be a multiple of 16, up to 512")
+    return dt
+
+
+def _append_fp8(append_key, append_value, cv, sv, err_count, batch_indices=None, positions=None, kv_indices=None,
+                kv_indptr=None, slots=None) -> None:
+    """The append into an 8-bit cache, by page table or slots."""
+    dev, dt = cv.device, _row_dtype(append_key, cv)
     nnz = append_key.shape[0]
-    _rows_fp8(append_key, append_value, cv, nnz)
-    ids = dict(zip(("batch_indices", "positions", "kv_indices", "kv_indptr"), table)) if table else {"slots": slots}
-    for n, t in ids.items():
-        if _i32(t, n).device != cv.device:
-            raise ValueError(f"{n} is on {t.device}, the cache on {cv.device}")
-    if any(t.numel() < nnz for n, t in ids.items() if not n.startswith("kv_")):
-        raise ValueError("append_key, append_value and " + (" and ".join(n for n in ids if not n.startswith("kv_")))
-                         + " disagree on nnz")
-    if table and ids["kv_indptr"].numel() < 1:
-        raise ValueError("kv_indptr must have batch+1 entries")
-    ksn, ksh = _row_strides(append_key, "append_key")
-    vsn, vsh = _row_strides(append_value, "append_value")
+    shape = (nnz, cv.num_kv_heads, cv.head_dim)
+    ks, vs = _rows(append_key, "append_key", shape, dt, dev), _rows(append_value, "append_value", shape, dt, dev)
+    if slots is not None:
+        table = (0, 0, _ids(slots, "slots", dev))
+        if slots.numel() < nnz:
+            raise ValueError("append_key, append_value and slots disagree on nnz")
+        idx, nidx, ptr, batch = 0, 0, 0, 0
+    else:
+        table = (_ids(batch_indices, "batch_indices", dev), _ids(positions, "positions", dev), 0)
+        if batch_indices.numel() < nnz or positions.numel() < nnz:
+            raise ValueError("append_key, append_value, batch_indices and positions disagree on nnz")
+        idx, nidx = _ids(kv_indices, "kv_indices", dev), kv_indices.numel()
+        ptr, batch = _ids(kv_indptr, "kv_indptr", dev), kv_indptr.numel() - 1
+        if batch < 0:
+            raise ValueError("kv_indptr must have batch+1 entries")
     err_ptr = _i32(err_count, "err_count").data_ptr() if err_count is not None else 0
     if nnz == 0:
         return
-    ptr = {n: t.data_ptr() for n, t in ids.items()}
-    check(lib().pkv_append_paged_kv_cache_fp8(
-        append_key.data_ptr(), ksn, ksh, append_value.data_ptr(), vsn, vsh, ptr.get("batch_indices", 0),
-        ptr.get("positions", 0), ptr.get("slots", 0), nnz, cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages,
-        sv.k_ptr, sv.v_ptr, sv.page_stride, ptr.get("kv_indices", 0),
-        ids["kv_indices"].numel() if table else 0, ptr.get("kv_indptr", 0),
-        ids["kv_indptr"].numel() - 1 if table else 0, cv.num_kv_heads, cv.head_dim, cv.page_size,
-        dtype_code(append_key.dtype), err_ptr, stream_ptr(cv.device)), "append_paged_kv_cache (8-bit cache)")
-
-
-def _rows_fp8(append_key, append_value, cv, nnz) -> None:
-    """Checks of the rows that go into an 8-bit cache."""
-    if append_key.dtype not in (torch.float16, torch.bfloat16, torch.float32) or append_value.dtype != append_key.dtype:
-        raise ValueError("append_key and append_value must share one of float16, bfloat16 and float32")
-    for t, n in ((append_key, "append_key"), (append_value, "append_value")):
-        if tuple(t.shape) != (nnz, cv.num_kv_heads, cv.head_dim):
-            raise ValueError(f"{n} must be [{nnz}, {cv.num_kv_heads}, {cv.head_dim}]")
-        if t.device != cv.device:
-            raise ValueError(f"{n} is on {t.device}, the cache on {cv.device}")
-    _head_dim_16(cv)
-
-
-def _head_dim_16(cv) -> None:
-    if cv.head_dim % 16 or not 0 < cv.head_dim <= 512:
-        raise ValueError("head_dim must be a multiple of 16, up to 512")
+    check(call(CALL_APPEND_FP8, append_key.data_ptr(), ks[0], ks[1], append_value.data_ptr(), vs[0], vs[1], *table, nnz,
+               cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages, sv.k_ptr, sv.v_ptr, sv.page_stride, idx, nidx, ptr, batch,
+               cv.num_kv_heads, cv.head_dim, cv.page_size, DTYPE_CODE[dt], err_ptr, stream_ptr(dev)),
+          "append_paged_kv_cache (8-bit cache)")
 
 
 def append_paged_kv_cache_slots(append_key: torch.Tensor, append_value: torch.Tensor, slots: torch.Tensor,
@@ -371,59 +394,61 @@ def append_paged_kv_cache_with_norm_rope(q: torch.Tensor, append_key: torch.Tens
     """
     cv = CacheView(paged_kv_cache, kv_layout)
     sv = ScaleView(kv_scales, cv) if cv.dtype == FP8 or kv_scales is not None else None
-    nnz, d, dt = append_key.shape[0], cv.head_dim, append_key.dtype
-    _rows_fp8(append_key, append_value, cv, nnz)
+    dev, dt, d = cv.device, _row_dtype(append_key, cv), cv.head_dim
     if sv is None and dt != cv.dtype:
         raise ValueError(f"append_key dtype {dt} differs from the cache dtype {cv.dtype}")
-    if q.dtype != dt or q.dim() != 3 or q.shape[0] != nnz or q.shape[2] != d:
+    nnz = append_key.shape[0]
+    shape = (nnz, cv.num_kv_heads, d)
+    ks, vs = _rows(append_key, "append_key", shape, dt, dev), _rows(append_value, "append_value", shape, dt, dev)
+    qshape = q.shape
+    if len(qshape) != 3 or qshape[0] != nnz or qshape[2] != d:
         raise ValueError(f"q must be [{nnz}, Hq, {d}] in {dt}")
-    for a, b, shape, names in ((q_weight, k_weight, (d,), ("q_weight", "k_weight")), (cos, sin, (nnz, d), ("cos", "sin"))):
-        for t, n in zip((a, b), names):
-            if t is None and shape == (d,):
-                continue
-            if not isinstance(t, torch.Tensor) or t.dtype not in (dt, torch.float32) or tuple(t.shape) != shape or \
-                    (t.numel() and t.stride(-1) != 1):
-                raise ValueError(f"{n} must be {list(shape)} in {dt} or float32 with a unit inner stride")
-        if a is not None and b is not None and a.dtype != b.dtype:
-            raise ValueError(f"{names[0]} and {names[1]} must share one dtype")
-    if cos.stride(0) != sin.stride(0):
-        raise ValueError("cos and sin must share a row stride")
+    qs = _rows(q, "q", qshape, dt, dev)
+    if q_out is None:
+        q_out = torch.empty_like(q) if q.is_contiguous() else torch.empty(qshape, dtype=dt, device=dev)
+        os = q_out.stride()
+    else:
+        os = _rows(q_out, "q_out", qshape, dt, dev)
+    qw = kw = 0
+    wdt = None
+    for t, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.shape != (d,) or t.stride(0) != 1 or t.dtype not in (dt, torch.float32):
+            raise ValueError(f"{n} must be [{d}] in {dt} or float32 with a unit inner stride")
+        if wdt is not None and t.dtype != wdt:
+            raise ValueError("q_weight and k_weight must share one dtype")
+        if t.device != dev:
+            raise ValueError(f"{n} is on {t.device}, the cache on {dev}")
+        wdt = t.dtype
+        if n == "q_weight":
+            qw = t.data_ptr()
+        else:
+            kw = t.data_ptr()
+    cdt, cst = cos.dtype, cos.stride()
+    for t, n in ((cos, "cos"), (sin, "sin")):
+        if t.shape != (nnz, d) or (nnz and t.stride() != cst) or cst[-1] != 1 or t.dtype != cdt or cdt not in (dt, torch.float32):
+            raise ValueError(f"cos and sin must both be [{nnz}, {d}] in {dt} or float32, with one row stride and a unit inner one")
+        if t.device != dev:
+            raise ValueError(f"{n} is on {t.device}, the cache on {dev}")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    _i32(batch_indices, "batch_indices")
-    _i32(positions, "positions")
-    _i32(kv_indices, "kv_indices")
-    _i32(kv_indptr, "kv_indptr")
+    bi, po = _ids(batch_indices, "batch_indices", dev), _ids(positions, "positions", dev)
     if batch_indices.numel() < nnz or positions.numel() < nnz:
         raise ValueError("q, append_key, append_value, batch_indices and positions disagree on nnz")
-    if kv_indptr.numel() < 1:
+    idx, ptr, batch = _ids(kv_indices, "kv_indices", dev), _ids(kv_indptr, "kv_indptr", dev), kv_indptr.numel() - 1
+    if batch < 0:
         raise ValueError("kv_indptr must have batch+1 entries")
-    if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif q_out.shape != q.shape or q_out.dtype != q.dtype:
-        raise ValueError("q_out must match q's shape and dtype")
-    qsn, qsh = _row_strides(q, "q")
-    osn, osh = _row_strides(q_out, "q_out")
-    ksn, ksh = _row_strides(append_key, "append_key")
-    vsn, vsh = _row_strides(append_value, "append_value")
-    for t, n in ((q, "q"), (q_out, "q_out"), (q_weight, "q_weight"), (k_weight, "k_weight"), (cos, "cos"), (sin, "sin"),
-                 (batch_indices, "batch_indices"), (positions, "positions"), (kv_indices, "kv_indices"),
-                 (kv_indptr, "kv_indptr")):
-        if t is not None and t.device != cv.device:
-            raise ValueError(f"{n} is on {t.device}, the cache on {cv.device}")
     err_ptr = _i32(err_count, "err_count").data_ptr() if err_count is not None else 0
     if nnz == 0:
         return q_out
-    w = q_weight if q_weight is not None else k_weight
-    check(lib().pkv_append_paged_kv_cache_norm_rope(
-        q.data_ptr(), qsn, qsh, q_out.data_ptr(), osn, osh, q.shape[1], append_key.data_ptr(), ksn, ksh,
-        append_value.data_ptr(), vsn, vsh, q_weight.data_ptr() if q_weight is not None else 0,
-        k_weight.data_ptr() if k_weight is not None else 0, dtype_code(w.dtype if w is not None else dt), float(eps),
-        cos.data_ptr(), sin.data_ptr(), cos.stride(0), dtype_code(cos.dtype), batch_indices.data_ptr(),
-        positions.data_ptr(), nnz, cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages, sv.k_ptr if sv else 0,
-        sv.v_ptr if sv else 0, sv.page_stride if sv else 0, kv_indices.data_ptr(), kv_indices.numel(),
-        kv_indptr.data_ptr(), kv_indptr.numel() - 1, cv.num_kv_heads, d, cv.page_size, dtype_code(dt), err_ptr,
-        stream_ptr(cv.device)), "append_paged_kv_cache_with_norm_rope")
+    code = DTYPE_CODE[dt]
+    scales = (sv.k_ptr, sv.v_ptr, sv.page_stride) if sv is not None else (0, 0, 0)
+    check(call(CALL_NORM_ROPE, q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), os[0], os[1], qshape[1], append_key.data_ptr(),
+               ks[0], ks[1], append_value.data_ptr(), vs[0], vs[1], qw, kw, code if wdt is None else DTYPE_CODE[wdt], float(eps),
+               cos.data_ptr(), sin.data_ptr(), cst[0], DTYPE_CODE[cdt], bi, po, nnz, cv.k_ptr, cv.v_ptr, cv.page_stride,
+               cv.num_pages, *scales, idx, kv_indices.numel(), ptr, batch, cv.num_kv_heads, d, cv.page_size, code, err_ptr,
+               stream_ptr(dev)), "append_paged_kv_cache_with_norm_rope")
     return q_out
 
 
@@ -438,24 +463,21 @@ def read_paged_kv_cache(paged_kv_cache: CacheT, kv_scales, kv_indices: torch.Ten
     """
     cv = CacheView(paged_kv_cache, kv_layout)
     sv = ScaleView(kv_scales, cv)
-    _head_dim_16(cv)
-    _i32(kv_indices, "kv_indices")
-    _i32(kv_indptr, "kv_indptr")
-    if kv_indptr.numel() < 1:
+    dev, d = cv.device, cv.head_dim
+    if d % 16 or not 0 < d <= 512:
+        raise ValueError("head_dim must be a multiple of 16, up to 512")
+    idx, ptr, batch = _ids(kv_indices, "kv_indices", dev), _ids(kv_indptr, "kv_indptr", dev), kv_indptr.numel() - 1
+    if batch < 0:
         raise ValueError("kv_indptr must have batch+1 entries")
-    if kv_indices.device != cv.device or kv_indptr.device != cv.device:
-        raise ValueError("kv_indices and kv_indptr must be on the cache's device")
     code = dtype_code(dtype)
     n = kv_indices.numel()
-    shape = (n, 2, cv.page_size, cv.num_kv_heads, cv.head_dim)
+    shape = (n, 2, cv.page_size, cv.num_kv_heads, d)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=cv.device)
-    elif tuple(out.shape) != shape or out.dtype != dtype or not out.is_contiguous() or out.device != cv.device:
+        out = torch.empty(shape, dtype=dtype, device=dev)
+    elif out.shape != shape or out.dtype != dtype or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"out must be {list(shape)} in {dtype}, contiguous, on the cache's device")
-    if n == 0 or kv_indptr.numel() == 1:
+    if n == 0 or batch == 0:
         return out
-    check(lib().pkv_read_paged_kv_cache_fp8(
-        cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages, sv.k_ptr, sv.v_ptr, sv.page_stride, kv_indices.data_ptr(),
-        n, kv_indptr.data_ptr(), kv_indptr.numel() - 1, cv.num_kv_heads, cv.head_dim, cv.page_size, out.data_ptr(),
-        code, stream_ptr(cv.device)), "read_paged_kv_cache")
+    check(call(CALL_READ_FP8, cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages, sv.k_ptr, sv.v_ptr, sv.page_stride, idx, n, ptr,
+               batch, cv.num_kv_heads, d, cv.page_size, out.data_ptr(), code, stream_ptr(dev)), "read_paged_kv_cache")
     return out

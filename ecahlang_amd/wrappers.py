@@ -24,7 +24,7 @@ import numpy as np
 
 import torch
 
-from ._lib import check, dtype_code, lib, stream_ptr
+from ._lib import CALL_DECODE_FP8, DTYPE_CODE, call, check, dtype_code, lib, stream_ptr
 from .ops import FP8, CacheView, ScaleView, _i32, read_paged_kv_cache
 
 _STR_DTYPES = {"float8_e4m3fn": FP8, "float16": torch.float16, "half": torch.float16, "bfloat16": torch.bfloat16,
@@ -59,6 +59,7 @@ def _unsupported(pos_encoding_mode, window_left, logits_soft_cap, rope_scale, ro
 _DECODE_VALU, _DECODE_DYNAMIC, _DECODE_PLANNED, _DECODE_HEAD_COUNTERS = 1, 2, 4, 8  # pkv_batch_decode flags (include/pagedkv.h)
 _PLAN_CASCADE = 1  # pkv_decode_plan flag
 _MAX_HEAD_COUNTERS = 2048  # PKV_MAX_HEAD_COUNTERS
+_PLAN_SEQS, _PLAN_TOKENS = 4096, 32768  # 8-bit caches: batches up to so many sequences are planned, from so many tokens x KV heads
 _INIT_COUNTERS = 8192  # decode split counters zeroed when a workspace is given
 
 class BatchDecodeWithPagedKVCacheWrapper:
@@ -208,8 +209,9 @@ class BatchDecodeWithPagedKVCacheWrapper:
         self._planned = True
 
     def _plan_fp8(self, dev: torch.device, num_ctas: int | None) -> None:
-        """An 8-bit cache's decode needs no schedule (it reads the page table when it runs): room for its
-        partials, and zeroed counters, one a sequence and block of 16 query heads of a KV head."""
+        """An 8-bit cache's decode reads the page table when it runs.  It needs room for its partials, zeroed
+        counters, one a sequence and block of 16 query heads of a KV head, and, for a batch of some length, how
+        long the parts of its sequences should be, from their lengths now (one small launch)."""
         if self._d not in (64, 128, 256):
             raise ValueError("head_dim must be 64, 128 or 256 for a float8_e4m3fn cache")
         if self._batch < 1 or self._ps < 1:
@@ -219,7 +221,8 @@ class BatchDecodeWithPagedKVCacheWrapper:
         if self._ctas <= 0:
             raise ValueError("num_ctas must be positive")
         ws = self._workspace
-        need = lib().pkv_decode_fp8_workspace_bytes(self._batch, self._hq, self._hkv, self._d, self._ctas)
+        pages = self._indices.numel()
+        need = lib().pkv_decode_fp8_workspace_bytes(self._batch, self._hq, self._hkv, self._d, self._ps, self._ctas, pages)
         if need < 0:
             check(int(need), "decode plan")
         if need > ws.numel() * ws.element_size():
@@ -228,19 +231,41 @@ class BatchDecodeWithPagedKVCacheWrapper:
         if counters > self._counters_ready:
             check(lib().pkv_decode_workspace_init(ws.data_ptr(), counters, stream_ptr(dev)), "decode plan")
         self._counters_ready = counters  # (the words after these are overwritten)
+        if self._batch <= _PLAN_SEQS and pages * self._ps * self._hkv > _PLAN_TOKENS:
+            check(lib().pkv_decode_fp8_plan(
+                self._indptr.data_ptr(), pages, self._last.data_ptr(), self._batch, self._hq, self._hkv, self._d, self._ps,
+                self._ctas, ws.data_ptr(), ws.numel() * ws.element_size(), stream_ptr(dev)), "decode plan")
+            self._flags = _DECODE_PLANNED
+        self._args = (self._indptr.data_ptr(), self._indices.data_ptr(), pages, self._last.data_ptr(), self._batch, self._hq,
+                      self._hkv, self._d, self._ps, self._sm_scale, self._ctas)
         self._planned = True
 
-    def _run_fp8(self, q: torch.Tensor, cv: CacheView, kv_scales, out: torch.Tensor) -> torch.Tensor:
+    def _run_fp8(self, q: torch.Tensor, paged_kv_cache, kv_scales, out: torch.Tensor | None) -> torch.Tensor:
+        cv = CacheView(paged_kv_cache, self._kv_layout)
+        dt, qs, ws = self._q_dtype, q.stride(), self._workspace
+        if q.dtype != dt or cv.dtype != FP8:
+            raise ValueError(f"q dtype must be {dt}, cache dtype {FP8}")
+        if q.shape != (self._batch, self._hq, self._d) or qs[2] != 1:
+            raise ValueError(f"q must be [{self._batch}, {self._hq}, {self._d}] with unit inner stride")
+        if (cv.num_kv_heads, cv.head_dim, cv.page_size) != (self._hkv, self._d, self._ps):
+            raise ValueError("cache geometry differs from plan()")
         sv = ScaleView(kv_scales, cv)
-        if (q.data_ptr() | q.stride(0) * 2 | q.stride(1) * 2) % 16:  # (rows are read 16 bytes at a time)
+        if q.device != cv.device:
+            raise ValueError(f"q is on {q.device}, the cache on {cv.device}")
+        if out is None:
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=cv.device)
+            st = out.stride()
+        else:
+            st = out.stride()
+            if out.shape != q.shape or out.dtype != dt or st[2] != 1 or out.device != cv.device:
+                raise ValueError("out must match q's shape, dtype and device")
+        qp = q.data_ptr()
+        if (qp | qs[0] * 2 | qs[1] * 2) % 16:  # (rows are read 16 bytes at a time)
             q = q.clone(memory_format=torch.contiguous_format)
-        check(lib().pkv_batch_decode_fp8(
-            q.data_ptr(), q.stride(0), q.stride(1), cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages, sv.k_ptr, sv.v_ptr,
-            sv.page_stride, self._indptr.data_ptr(), self._indices.data_ptr(), self._indices.numel(),
-            self._last.data_ptr(), self._batch, self._hq, self._hkv, self._d, self._ps, self._sm_scale, self._ctas,
-            self._workspace.data_ptr(), self._workspace.numel() * self._workspace.element_size(), out.data_ptr(),
-            out.stride(0), out.stride(1), dtype_code(q.dtype), stream_ptr(q.device)),
-            "BatchDecodeWithPagedKVCacheWrapper.run")
+            qp, qs = q.data_ptr(), q.stride()
+        check(call(CALL_DECODE_FP8, qp, qs[0], qs[1], cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages, sv.k_ptr, sv.v_ptr,
+                   sv.page_stride, *self._args, ws.data_ptr(), ws.numel() * ws.element_size(), out.data_ptr(), st[0], st[1],
+                   DTYPE_CODE[dt], self._flags, stream_ptr(cv.device)), "BatchDecodeWithPagedKVCacheWrapper.run")
         return out
 
     def run(self, q: torch.Tensor, paged_kv_cache, *args, q_scale=None, k_scale=None,
@@ -254,6 +279,14 @@ class BatchDecodeWithPagedKVCacheWrapper:
         scales of a float8_e4m3fn cache (``ops.ScaleView``)."""
         if not self._planned:
             raise RuntimeError("plan() must be called before run()")
+        if self._fp8:
+            if return_lse or lse is not None:
+                raise NotImplementedError("return_lse is not implemented")
+            if q_scale is not None or k_scale is not None or v_scale is not None:
+                raise NotImplementedError("a float8_e4m3fn cache's scales are kv_scales")
+            if append_kv is not None or force_valu:
+                raise NotImplementedError("append_kv and force_valu are not implemented for float8_e4m3fn caches")
+            return self._run_fp8(q, paged_kv_cache, kv_scales, out)
         if torch.cuda.is_current_stream_capturing():
             self._captured_mode = self._cascade_mode
         if return_lse or lse is not None:
@@ -263,18 +296,14 @@ class BatchDecodeWithPagedKVCacheWrapper:
         cv = CacheView(paged_kv_cache, self._kv_layout)
         if q.dim() != 3 or q.shape != (self._batch, self._hq, self._d) or q.stride(2) != 1:
             raise ValueError(f"q must be [{self._batch}, {self._hq}, {self._d}] with unit inner stride")
-        if q.dtype != self._q_dtype or cv.dtype != self._kv_dtype:
-            raise ValueError(f"q dtype must be {self._q_dtype}, cache dtype {self._kv_dtype}")
+        if q.dtype != self._q_dtype or cv.dtype != self._q_dtype:
+            raise ValueError(f"q / cache dtype must be {self._q_dtype}")
         if (cv.num_kv_heads, cv.head_dim, cv.page_size) != (self._hkv, self._d, self._ps):
             raise ValueError("cache geometry differs from plan()")
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
             raise ValueError("out must match q's shape and dtype")
-        if self._fp8:
-            if append_kv is not None or force_valu:
-                raise NotImplementedError("append_kv and force_valu are not implemented for float8_e4m3fn caches")
-            return self._run_fp8(q, cv, kv_scales, out)
         if kv_scales is not None:
             raise ValueError("kv_scales go with a float8_e4m3fn cache")
         if append_kv is not None:

@@ -156,13 +156,19 @@ int pkv_read_paged_kv_cache_fp8(const void* k_cache, const void* v_cache, int64_
                                 int32_t dtype, void* stream);
 
 /* Decode attention over an 8-bit cache: pkv_batch_decode's contract with fp16 or bf16 queries (`dtype`),
- * head_dim 64, 128 or 256, any page size and group.  No plan: the page table is read when the call
- * runs.  The workspace (pkv_decode_fp8_workspace_bytes) starts with batch * Hkv * ceil(group / 16)
- * arrival counters, zeroed once (pkv_decode_workspace_init of that many) and left at zero; it
- * belongs to one call at a time.  q rows, the caches and page_stride have to be multiples of 16
- * bytes, for a page_size that is a multiple of 16 the scales and their stride of 4. */
-int64_t pkv_decode_fp8_workspace_bytes(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
-                                       int32_t head_dim, int32_t num_ctas);
+ * head_dim 64, 128 or 256, any page size and group, up to 2^31 - 64 tokens that num_indices pages hold.
+ * The page table is read when the call runs.  The workspace (pkv_decode_fp8_workspace_bytes) starts
+ * with batch * Hkv * ceil(group / 16) arrival counters, zeroed once (pkv_decode_workspace_init of
+ * that many) and left at zero; it belongs to one call at a time.  q rows, the caches and page_stride
+ * have to be multiples of 16 bytes, for a page_size that is a multiple of 16 the scales and their
+ * stride of 4.  pkv_decode_fp8_plan (optional; batch <= 4096; one small launch) writes into the
+ * workspace how long a part of a sequence should be for these lengths, which calls with `flags`
+ * PKV_DECODE_PLANNED and the same sizes then use; a plan for other lengths costs time, nothing else. */
+int64_t pkv_decode_fp8_workspace_bytes(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+                                       int32_t page_size, int32_t num_ctas, int64_t num_indices);
+int pkv_decode_fp8_plan(const int32_t* kv_indptr, int64_t num_indices, const int32_t* kv_last_page_len,
+                        int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+                        int32_t page_size, int32_t num_ctas, void* workspace, int64_t workspace_bytes, void* stream);
 int pkv_batch_decode_fp8(const void* q, int64_t q_stride_n, int64_t q_stride_h, const void* k_cache,
                          const void* v_cache, int64_t page_stride, int64_t num_pages, const void* k_scales,
                          const void* v_scales, int64_t scale_page_stride, const int32_t* kv_indptr,
@@ -170,7 +176,15 @@ int pkv_batch_decode_fp8(const void* q, int64_t q_stride_n, int64_t q_stride_h, 
                          int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
                          int32_t page_size, float sm_scale, int32_t num_ctas, void* workspace,
                          int64_t workspace_bytes, void* out, int64_t o_stride_n, int64_t o_stride_h,
-                         int32_t dtype, void* stream);
+                         int32_t dtype, int32_t flags, void* stream);
+
+/* One of the entry points above with its arguments as `count` 8-byte words, in order (integers and pointers as
+ * int64, floats as double): for bindings that pay for every argument they convert. */
+#define PKV_CALL_APPEND_FP8 0 /* pkv_append_paged_kv_cache_fp8 */
+#define PKV_CALL_NORM_ROPE 1  /* pkv_append_paged_kv_cache_norm_rope */
+#define PKV_CALL_READ_FP8 2   /* pkv_read_paged_kv_cache_fp8 */
+#define PKV_CALL_DECODE_FP8 3 /* pkv_batch_decode_fp8 */
+int pkv_call(int32_t entry, const void* words, int32_t count);
 
 /* Smallest workspace pkv_decode_plan and pkv_batch_decode need for this geometry (num_indices =
  * length of the kv_indices buffer): the host half of BatchDecodeWithPagedKVCacheWrapper.plan
