@@ -10,9 +10,14 @@
 // all in fp32 and rounded once, to the type of q_out or the cache, or to e4m3 with the row's scale
 // (cache_fp8.h).  Without a weight the rows are not normalised.  Value rows are copied, or rounded to e4m3.
 //
-// A wave takes rows of one token: a group of D / 16 lanes (rounded up to a power of two) a row, each lane 8
-// elements of either half, so the rotation's partners meet in one lane and the sum of squares takes a few
-// lane exchanges.
+// A group of D / 16 lanes (rounded up to a power of two) takes a row, each lane 8 elements of either half, so
+// the rotation's partners meet in one lane and the sum of squares takes a few lane exchanges.  The rows of all
+// tokens are dealt out in one run, 8 of 128 dims to a wave, whatever the heads of a token are: a wave that kept
+// to one token, its angles in registers, idled lanes wherever the heads do not divide by 8 and waited for each
+// token's page by itself (4003 tokens, 32 / 8 heads of 128: 20 us for 30, a step of 4 tokens 3.0 for 4.8).
+//
+// What bounds it: the bytes, beside some 250 vector instructions a wave's 8 rows, about half the time at full
+// rate: 16,003 tokens, 32 / 8 heads of 128, bf16 into 8 bits, 80 us for 369 MB (71 at the rate of a large copy).
 #include "cache_fp8.h"
 #include "../../include/pagedkv.h"
 
@@ -23,118 +28,127 @@ using namespace pkv::fp8;
 
 namespace {
 
+// Workgroups at most: more of them than the chip holds at once (1280), so that their phases mix (the bulk above: 88 us
+// with 1024 or 2048, 83 with 4096, 79 with 8192, 81 with 16,384; a workgroup costs some 3.5 ns to start).
+constexpr int kGrid = 8192;
+
 struct NormRopeArgs {
   const void* q;
-  int64_t q_sn, q_sh;
   void* q_out;
-  int64_t qo_sn, qo_sh;
   const void *k, *v;
-  int64_t k_sn, k_sh, v_sn, v_sh;
+  Strides qs, os, ks, vs;
   const void *qw, *kw;  // null: that kind of row is not normalised
   const void *cos, *sin;
-  int64_t cs_sn;
+  Strides cs;
   float eps;
   Table t;
   Dest o;
-  int32_t nnz, hq, hkv, d, lanes, splits, w_f32, cs_f32;
+  Div rows;
+  int32_t nnz, hq, hkv, d, lanes, w_f32, cs_f32;
   int32_t* err;
 };
 
-// 8 weights or angles, of the rows' type or fp32 (wave-uniform).
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8f(const void* p, int64_t at, bool f32, float (&x)[8]) {
-  if (f32) {
-    Eight<float, VEC> r;
-    r.load((const float*)p + at);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = r.e[j];
-  } else {
-    Eight<T, VEC> r;
-    r.load((const T*)p + at);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = to_f32(r.e[j]);
+// 8 weights or angles: of the rows' type, or (MIXED) of that or fp32 as the call says.
+template <typename T, bool VEC, bool MIXED>
+struct Coef {
+  Eight<T, VEC> r;
+  Eight<float, VEC> f;
+  // 8 at element `at` of p
+  __device__ __forceinline__ void load(const void* p, int at, bool f32) {
+    if (MIXED && f32) f.load((const float*)p + at);
+    else r.load((const T*)p + at);
   }
-}
+  __device__ __forceinline__ void get(float (&x)[8], bool f32) const {
+    if (MIXED && f32) f.get(x);
+    else r.get(x);
+  }
+};
 
-template <typename T, bool QUANT, bool VEC>
-__global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a) {
+// Rows of all tokens in one run (token, then query, key and value heads): a group of lanes takes one row at a
+// time, wherever tokens end.  Everything a row needs is requested at once; only key and value rows look up
+// their page.
+template <typename T, bool QUANT, bool VEC, bool MIXED>
+__global__ __launch_bounds__(256, 4) void norm_rope_kernel(NormRopeArgs a) {
   const int lane = threadIdx.x & 63, sub = lane & (a.lanes - 1), per = 64 / a.lanes, half = a.d / 2;
   const bool act = 8 * sub < half;
   const int d0 = act ? 8 * sub : 0;
-  const int rows = a.hq + 2 * a.hkv;
-  const int gw = __builtin_amdgcn_readfirstlane(blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6));
-  const int nt = gridDim.x * (blockDim.x >> 6) / a.splits;  // tokens at a time
-  const int split = gw % a.splits;
-  for (int64_t tok = gw / a.splits; tok < a.nnz && gw < nt * a.splits; tok += nt) {
-    float c0[8], c1[8], s0[8], s1[8];
-    load8f<T, VEC>(a.cos, tok * a.cs_sn + d0, a.cs_f32, c0);
-    load8f<T, VEC>(a.cos, tok * a.cs_sn + d0 + half, a.cs_f32, c1);
-    load8f<T, VEC>(a.sin, tok * a.cs_sn + d0, a.cs_f32, s0);
-    load8f<T, VEC>(a.sin, tok * a.cs_sn + d0 + half, a.cs_f32, s1);
+  const uint32_t total = (uint32_t)a.nnz * a.rows.d;
+  const uint32_t stride = gridDim.x * (blockDim.x >> 6) * per;
+  const float inv_d = 1.f / (float)a.d;
+  uint32_t base = __builtin_amdgcn_readfirstlane((blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6)) * per);
+  for (; base < total; base += stride) {
+    const uint32_t at = base + lane / a.lanes, idx = at < total ? at : total - 1;
+    const uint32_t tok = a.rows.of(idx);
+    const int row = idx - tok * a.rows.d;
+    const bool isq = row < a.hq, isv = row >= a.hq + a.hkv, in = at < total && act;
+    const int h = isq ? row : (isv ? row - a.hq - a.hkv : row - a.hq);
+    const Strides st{isq ? a.qs.n : isv ? a.vs.n : a.ks.n, isq ? a.qs.h : isv ? a.vs.h : a.ks.h};
+    const T* src = (const T*)row_at(isq ? a.q : isv ? a.v : a.k, st, tok, h) + d0;
+    Eight<T, VEC> lo, hi;
+    lo.load(src);
+    hi.load(src + half);
+    const void *cosr = row_at(a.cos, a.cs, tok, 0), *sinr = row_at(a.sin, a.cs, tok, 0);
+    Coef<T, VEC, MIXED> c0, c1, s0, s1;
+    c0.load(cosr, d0, a.cs_f32);
+    c1.load(cosr, d0 + half, a.cs_f32);
+    s0.load(sinr, d0, a.cs_f32);
+    s1.load(sinr, d0 + half, a.cs_f32);
+    asm volatile("" ::: "memory");
     int page = 0, slot = 0;
-    const bool ok = resolve(a.t, tok, page, slot);
-    if (!ok && split == 0 && lane == 0 && a.err) atomicAdd(a.err, 1);
-    for (int r0 = split * per; r0 < rows; r0 += a.splits * per) {
-      const int rr = r0 + lane / a.lanes, row = rr < rows ? rr : rows - 1;
-      const bool isq = row < a.hq, isv = row >= a.hq + a.hkv;
-      const int h = isq ? row : (isv ? row - a.hq - a.hkv : row - a.hq);
-      const T* src = isq ? (const T*)a.q + tok * a.q_sn + h * a.q_sh
-                         : (isv ? (const T*)a.v + tok * a.v_sn + h * a.v_sh : (const T*)a.k + tok * a.k_sn + h * a.k_sh);
-      Eight<T, VEC> lo, hi;
-      lo.load(src + d0);
-      hi.load(src + d0 + half);
-      float x[8], y[8];
+    bool ok = false;
+    if (!isq) {
+      ok = resolve(a.t, tok, page, slot);
+      if (!ok && at < total && row == a.hq && sub == 0 && a.err) atomicAdd(a.err, 1);
+    }
+    float x[8], y[8];
+    lo.get(x);
+    hi.get(y);
+    if (__ballot(!isv)) {
       float ss = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = to_f32(lo.e[j]), y[j] = to_f32(hi.e[j]);
-        ss += x[j] * x[j] + y[j] * y[j];
-      }
+      for (int j = 0; j < 8; ++j) ss += x[j] * x[j] + y[j] * y[j];
       ss = group_sum(act ? ss : 0.f, a.lanes);
       if (!isv) {
         const void* w = isq ? a.qw : a.kw;
         if (w) {
-          const float rs = 1.f / sqrtf(ss / (float)a.d + a.eps);
-          float w0[8], w1[8];
-          load8f<T, VEC>(w, d0, a.w_f32, w0);
-          load8f<T, VEC>(w, d0 + half, a.w_f32, w1);
+          const float rs = __builtin_amdgcn_rsqf(ss * inv_d + a.eps);
+          Coef<T, VEC, MIXED> w0, w1;
+          w0.load(w, d0, a.w_f32);
+          w1.load(w, d0 + half, a.w_f32);
+          float u[8];
+          w0.get(u, a.w_f32);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = x[j] * rs * w0[j], y[j] = y[j] * rs * w1[j];
-        }
+          for (int j = 0; j < 8; ++j) x[j] *= rs * u[j];
+          w1.get(u, a.w_f32);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float u = x[j] * c0[j] - y[j] * s0[j], z = y[j] * c1[j] + x[j] * s1[j];
-          x[j] = u, y[j] = z;
-          lo.e[j] = from_f32<T>(u), hi.e[j] = from_f32<T>(z);
+          for (int j = 0; j < 8; ++j) y[j] *= rs * u[j];
         }
+        float c[8], s[8], z[8];
+        c0.get(c, a.cs_f32);
+        s0.get(s, a.cs_f32);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = x[j] * c[j] - y[j] * s[j];
+        c1.get(c, a.cs_f32);
+        s1.get(s, a.cs_f32);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = y[j] * c[j] + x[j] * s[j], x[j] = z[j];
+        if (!QUANT || isq) lo.set(x), hi.set(y);
       }
-      const bool in = rr < rows && act;
-      int e = 0;
-      if constexpr (QUANT) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = amax_bits(amax_bits(m, x[j]), y[j]);
-        e = scale_byte(group_max(act ? m : 0u, a.lanes));
-      }
-      if (isq) {
-        if (in) {
-          T* dst = (T*)a.q_out + tok * a.qo_sn + h * a.qo_sh + d0;
-          lo.store(dst);
-          hi.store(dst + half);
-        }
-      } else if (in && ok) {
-        const int64_t at = page * a.o.page_stride + ((int64_t)slot * a.hkv + h) * a.d + d0;
-        if constexpr (QUANT) {
-          uint8_t* dst = (uint8_t*)(isv ? a.o.v : a.o.k) + at;
-          const float inv = inv_scale(e);
-          store8<VEC>(dst, x, inv);
-          store8<VEC>(dst + half, y, inv);
-          if (sub == 0) (isv ? a.o.vs : a.o.ks)[page * a.o.scale_stride + (int64_t)h * a.t.ps + slot] = (uint8_t)e;
-        } else {
-          T* dst = (T*)(isv ? a.o.v : a.o.k) + at;
-          lo.store(dst);
-          hi.store(dst + half);
-        }
+    }
+    if (in && (isq || (!QUANT && ok))) {
+      T* dst = (isq ? (T*)row_at(a.q_out, a.os, tok, h)
+                    : (T*)(isv ? a.o.v : a.o.k) + page * a.o.page_stride + (uint32_t)((slot * a.hkv + h) * a.d)) + d0;
+      lo.store(dst, !isq);
+      hi.store(dst + half, !isq);
+    }
+    if (QUANT && __ballot(!isq)) {
+      const int e = row_scale(x, y, act, a.lanes);
+      if (in && ok) {
+        uint8_t* dst = (uint8_t*)(isv ? a.o.v : a.o.k) + page * a.o.page_stride + (uint32_t)((slot * a.hkv + h) * a.d + d0);
+        const float inv = inv_scale(e);
+        store8<VEC>(dst, x, inv);
+        store8<VEC>(dst + half, y, inv);
+        if (sub == 0) (isv ? a.o.vs : a.o.ks)[page * a.o.scale_stride + (h * a.t.ps.d + slot)] = (uint8_t)e;
       }
     }
   }
@@ -159,30 +173,35 @@ extern "C" int pkv_append_paged_kv_cache_norm_rope(
   const bool quant = k_scales != nullptr;
   if (quant != (v_scales != nullptr) || !cos || !sin || !batch_indices || !positions || !kv_indptr) return kBadArg;
   const int lanes = lanes_of(head_dim), per = 64 / lanes, rows = num_qo_heads + 2 * num_kv_heads;
-  // The waves a token's rows are shared by: all there is work for while tokens are few.
-  const int most = (rows + per - 1) / per;
-  const int64_t spread = (8192 + (int64_t)nnz - 1) / nnz;
-  const int splits = spread < most ? (int)spread : most;
-  const NormRopeArgs a{q, q_stride_n, q_stride_h, q_out, qo_stride_n, qo_stride_h, append_key, append_value, k_stride_n,
-                       k_stride_h, v_stride_n, v_stride_h, q_weight, k_weight, cos, sin, cs_stride_n, eps,
-                       {batch_indices, positions, nullptr, kv_indices, kv_indptr, num_indices, num_pages, batch, page_size},
+  const int64_t total = (int64_t)nnz * rows;
+  if (total > INT32_MAX) return kBadArg;
+  Strides qs, os, ks, vs, cs;
+  if (!strides_of(q_stride_n, q_stride_h, es, &qs) || !strides_of(qo_stride_n, qo_stride_h, es, &os) ||
+      !strides_of(k_stride_n, k_stride_h, es, &ks) || !strides_of(v_stride_n, v_stride_h, es, &vs) ||
+      !strides_of(cs_stride_n, 0, cs_dtype == kF32 ? 4 : es, &cs) || !page_fits(page_size, num_kv_heads, head_dim))
+    return kBadArg;
+  const NormRopeArgs a{q, q_out, append_key, append_value, qs, os, ks, vs, q_weight, k_weight, cos, sin, cs, eps,
+                       {batch_indices, positions, nullptr, kv_indices, kv_indptr, num_indices, num_pages, batch, Div(page_size)},
                        {k_cache, v_cache, (uint8_t*)k_scales, (uint8_t*)v_scales, page_stride, scale_page_stride},
-                       nnz, num_qo_heads, num_kv_heads, head_dim, lanes, splits,
-                       weight_dtype == kF32, cs_dtype == kF32, err_count};
+                       Div(rows), nnz, num_qo_heads, num_kv_heads, head_dim, lanes, weight_dtype == kF32, cs_dtype == kF32,
+                       err_count};
   const uintptr_t m = (uintptr_t)q | (uintptr_t)q_out | (uintptr_t)append_key | (uintptr_t)append_value;
-  const uintptr_t cs = (uintptr_t)cos | (uintptr_t)sin, ws = (uintptr_t)q_weight | (uintptr_t)k_weight;
+  const uintptr_t an = (uintptr_t)cos | (uintptr_t)sin, ws = (uintptr_t)q_weight | (uintptr_t)k_weight;
   const uintptr_t to = (uintptr_t)k_cache | (uintptr_t)v_cache;
-  if ((m % es) || cs % (cs_dtype == kF32 ? 4 : es) || ws % (weight_dtype == kF32 ? 4 : es) || (!quant && to % es)) return kBadAlign;
+  if ((m % es) || an % (cs_dtype == kF32 ? 4 : es) || ws % (weight_dtype == kF32 ? 4 : es) || (!quant && to % es)) return kBadAlign;
   const int64_t st = q_stride_n | q_stride_h | qo_stride_n | qo_stride_h | k_stride_n | k_stride_h | v_stride_n | v_stride_h;
-  const bool vec = (m | cs | ws) % 16 == 0 && st * es % 16 == 0 && cs_stride_n * (cs_dtype == kF32 ? 4 : es) % 16 == 0 &&
+  const bool vec = (m | an | ws) % 16 == 0 && st * es % 16 == 0 && cs_stride_n * (cs_dtype == kF32 ? 4 : es) % 16 == 0 &&
                    (quant ? to % 8 == 0 && page_stride % 8 == 0 : to % 16 == 0 && page_stride * es % 16 == 0);
-  const int64_t waves = (int64_t)nnz * splits, want = (waves + 3) / 4;
-  const dim3 grid((unsigned)(want < 16384 ? want : 16384));
+  const int64_t want = (total + 4 * per - 1) / (4 * per);
+  const dim3 grid((unsigned)(want < kGrid ? want : kGrid));
+  const bool mixed = weight_dtype != dtype || cs_dtype != dtype;
   hipStream_t s = (hipStream_t)stream;
-#define PKV_NORM_ROPE(T, Q, V) hipLaunchKernelGGL((norm_rope_kernel<T, Q, V>), grid, dim3(256), 0, s, a)
-#define PKV_NORM_ROPE_T(T)                                                         \
-  if (quant) { if (vec) PKV_NORM_ROPE(T, true, true); else PKV_NORM_ROPE(T, true, false); }    \
-  else { if (vec) PKV_NORM_ROPE(T, false, true); else PKV_NORM_ROPE(T, false, false); }
+#define PKV_NORM_ROPE(T, Q, V, M) hipLaunchKernelGGL((norm_rope_kernel<T, Q, V, M>), grid, dim3(256), 0, s, a)
+#define PKV_NORM_ROPE_Q(T, Q)                                                              \
+  if (vec) { if (mixed) PKV_NORM_ROPE(T, Q, true, true); else PKV_NORM_ROPE(T, Q, true, false); }   \
+  else { if (mixed) PKV_NORM_ROPE(T, Q, false, true); else PKV_NORM_ROPE(T, Q, false, false); }
+#define PKV_NORM_ROPE_T(T) \
+  if (quant) { PKV_NORM_ROPE_Q(T, true) } else { PKV_NORM_ROPE_Q(T, false) }
   if (dtype == kF16) {
     PKV_NORM_ROPE_T(_Float16)
   } else if (dtype == kBF16) {
@@ -191,6 +210,7 @@ extern "C" int pkv_append_paged_kv_cache_norm_rope(
     PKV_NORM_ROPE_T(float)
   }
 #undef PKV_NORM_ROPE_T
+#undef PKV_NORM_ROPE_Q
 #undef PKV_NORM_ROPE
   return (int)hipGetLastError();
 }

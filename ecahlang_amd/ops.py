@@ -36,76 +36,74 @@ class CacheView:
                  "head_dim", "dtype", "device")
 
     def __init__(self, paged_kv_cache: CacheT, kv_layout: str = "NHD"):
-        if kv_layout != "NHD" and kv_layout.upper() != "NHD":
-            raise NotImplementedError("only the NHD cache layout is implemented (the reference uses NHD)")
-        if isinstance(paged_kv_cache, (tuple, list)):
-            k, v = paged_kv_cache
-            if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
-                raise ValueError("(k_cache, v_cache) must both be [pages, page_size, Hkv, D]")
-            for t in (k, v):
-                if not t.is_contiguous():
-                    raise ValueError("k_cache / v_cache must be contiguous")
-            self.k_ptr, self.v_ptr = k.data_ptr(), v.data_ptr()
-            self.num_pages, self.page_size, self.num_kv_heads, self.head_dim = k.shape
-            self.page_stride = k.stride(0)
-        else:
-            k = paged_kv_cache
-            shape = k.shape
-            if len(shape) != 5 or shape[1] != 2:
-                raise ValueError("paged_kv_cache must be [pages, 2, page_size, Hkv, D] (NHD)")
-            if not k.is_contiguous():
-                raise ValueError("paged_kv_cache must be contiguous")
-            self.num_pages, _, self.page_size, self.num_kv_heads, self.head_dim = shape
-            self.k_ptr = p = k.data_ptr()
-            half = shape[2] * shape[3] * shape[4]
-            self.v_ptr = p + half * k.element_size() if p else 0
-            self.page_stride = 2 * half
-        self.dtype, self.device = k.dtype, k.device
-        if not k.is_cuda:
-            raise ValueError("paged_kv_cache must live on a CUDA (HIP) device")
+        (self.k_ptr, self.v_ptr, self.page_stride, self.num_pages, self.page_size, self.num_kv_heads, self.head_dim,
+         self.dtype, self.device) = cache_fields(paged_kv_cache, kv_layout)
+
+
+def cache_fields(paged_kv_cache: CacheT, kv_layout: str = "NHD") -> tuple:
+    """A ``CacheView``'s fields in order, for calls where the object's own time counts."""
+    if kv_layout != "NHD" and kv_layout.upper() != "NHD":
+        raise NotImplementedError("only the NHD cache layout is implemented (the reference uses NHD)")
+    if isinstance(paged_kv_cache, (tuple, list)):
+        k, v = paged_kv_cache
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("(k_cache, v_cache) must both be [pages, page_size, Hkv, D]")
+        for t in (k, v):
+            if not t.is_contiguous():
+                raise ValueError("k_cache / v_cache must be contiguous")
+        pages, ps, hkv, d = k.shape
+        kp, vp, stride = k.data_ptr(), v.data_ptr(), k.stride(0)
+    else:
+        k = paged_kv_cache
+        shape = k.shape
+        if len(shape) != 5 or shape[1] != 2:
+            raise ValueError("paged_kv_cache must be [pages, 2, page_size, Hkv, D] (NHD)")
+        if not k.is_contiguous():
+            raise ValueError("paged_kv_cache must be contiguous")
+        pages, _, ps, hkv, d = shape
+        kp = k.data_ptr()
+        half = ps * hkv * d
+        vp = kp + half * k.element_size() if kp else 0
+        stride = 2 * half
+    if not k.is_cuda:
+        raise ValueError("paged_kv_cache must live on a CUDA (HIP) device")
+    return kp, vp, stride, pages, ps, hkv, d, k.dtype, k.device
 
 
 FP8 = torch.float8_e4m3fn
 
 
-class ScaleView:
-    """Base pointers and page stride of an 8-bit cache's scales.
-
-    An 8-bit cache (``torch.float8_e4m3fn``, same shapes as the others) goes with one power-of-two
-    scale a token and KV head, ``torch.float8_e8m0fnu`` of shape ``[pages, 2, Hkv, page_size]``
-    (``new_kv_scales``), or a ``(k_scales, v_scales)`` pair of ``[pages, Hkv, page_size]`` for a
-    ``(k_cache, v_cache)`` pair.  A stored value is code * scale."""
-
-    __slots__ = ("k_ptr", "v_ptr", "page_stride")
-
-    def __init__(self, kv_scales, cv: CacheView):
-        if cv.dtype != FP8:
-            raise ValueError(f"kv_scales go with a float8_e4m3fn cache, not {cv.dtype}")
-        if kv_scales is None:
-            raise ValueError("a float8_e4m3fn cache needs kv_scales")
-        pages, ps, hkv = cv.num_pages, cv.page_size, cv.num_kv_heads
-        pair = isinstance(kv_scales, (tuple, list))
-        if pair and len(kv_scales) != 2:
+def scale_fields(kv_scales, pages: int, ps: int, hkv: int, dtype: torch.dtype, dev: torch.device) -> tuple:
+    """(K address, V address, bytes between pages) of the scales (``new_kv_scales``) of a cache of these sizes."""
+    if dtype is not FP8:
+        raise ValueError(f"kv_scales go with a float8_e4m3fn cache, not {dtype}")
+    if kv_scales is None:
+        raise ValueError("a float8_e4m3fn cache needs kv_scales")
+    if isinstance(kv_scales, (tuple, list)):
+        if len(kv_scales) != 2:
             raise ValueError("kv_scales must be one tensor or a (k_scales, v_scales) pair")
-        want = (pages, hkv, ps) if pair else (pages, 2, hkv, ps)
-        for t in kv_scales if pair else (kv_scales,):
-            if not isinstance(t, torch.Tensor) or t.dtype != torch.float8_e8m0fnu or t.shape != want:
-                raise ValueError(f"kv_scales must be float8_e8m0fnu {list(want)}")
-            if not t.is_contiguous():
-                raise ValueError("kv_scales must be contiguous")
-            if t.device != cv.device:
-                raise ValueError(f"kv_scales are on {t.device}, the cache on {cv.device}")
-        n = hkv * ps
-        if pair:
-            self.k_ptr, self.v_ptr, self.page_stride = kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), n
-        else:
-            self.k_ptr = p = kv_scales.data_ptr()
-            self.v_ptr, self.page_stride = p + n if p else 0, 2 * n
+        for t in kv_scales:
+            _check_scales(t, (pages, hkv, ps), dev)
+        return kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), hkv * ps
+    _check_scales(kv_scales, (pages, 2, hkv, ps), dev)
+    p, n = kv_scales.data_ptr(), hkv * ps
+    return p, p + n if p else 0, 2 * n
+
+
+def _check_scales(t, want: tuple, dev: torch.device) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.float8_e8m0fnu or t.shape != want:
+        raise ValueError(f"kv_scales must be float8_e8m0fnu {list(want)}")
+    if not t.is_contiguous():
+        raise ValueError("kv_scales must be contiguous")
+    if t.device != dev:
+        raise ValueError(f"kv_scales are on {t.device}, the cache on {dev}")
 
 
 def new_kv_scales(paged_kv_cache: torch.Tensor) -> torch.Tensor:
-    """Scales (of ones) for an 8-bit cache ``[..., pages, 2, page_size, Hkv, D]``: ``[..., pages, 2, Hkv,
-    page_size]``, ``torch.float8_e8m0fnu``."""
+    """Scales for an 8-bit cache (``torch.float8_e4m3fn``, same shapes as the others): one power of two a token and
+    KV head, ``torch.float8_e8m0fnu`` of shape ``[..., pages, 2, Hkv, page_size]`` for a cache ``[..., pages, 2,
+    page_size, Hkv, D]``, here of ones.  A stored value is code * scale.  With a ``(k_cache, v_cache)`` pair goes a
+    ``(k_scales, v_scales)`` pair of ``[pages, Hkv, page_size]``."""
     *lead, two, ps, hkv, _ = paged_kv_cache.shape
     if two != 2 or paged_kv_cache.dtype != FP8:
         raise ValueError("paged_kv_cache must be float8_e4m3fn [..., pages, 2, page_size, Hkv, D]")
@@ -167,15 +165,17 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor,
     dependency, not used by the scatter.  ``err_count`` (optional int32 [1]) counts tokens
     whose metadata falls outside their sequence's pages; they are skipped.
 
-    With an 8-bit cache (``torch.float8_e4m3fn``) and its ``kv_scales`` (see ``ScaleView``) the rows, fp16,
+    With an 8-bit cache (``torch.float8_e4m3fn``) and its ``kv_scales`` (see ``new_kv_scales``) the rows, fp16,
     bf16 or fp32, are quantised as they are written: each (token, head) row gets the smallest power of
     two s >= 2^-126 with max|x| <= 448 s as its scale and is stored as the e4m3 values nearest to x / s.
     Elements that are not finite are stored as NaN.  head_dim must be a multiple of 16, up to 512.
     """
-    cv = CacheView(paged_kv_cache, kv_layout)
-    if cv.dtype == FP8 or kv_scales is not None:
-        return _append_fp8(append_key, append_value, cv, ScaleView(kv_scales, cv), err_count, batch_indices, positions,
+    if kv_scales is not None:
+        return _append_fp8(append_key, append_value, paged_kv_cache, kv_layout, kv_scales, err_count, batch_indices, positions,
                            kv_indices, kv_indptr)
+    cv = CacheView(paged_kv_cache, kv_layout)
+    if cv.dtype is FP8:
+        raise ValueError("a float8_e4m3fn cache needs kv_scales")
     for t, n in ((append_key, "append_key"), (append_value, "append_value")):
         if t.dtype != cv.dtype:
             raise ValueError(f"{n} dtype {t.dtype} differs from the cache dtype {cv.dtype}")
@@ -206,7 +206,7 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor,
 
 def _ids(t: torch.Tensor, name: str, dev: torch.device) -> int:
     """Address of an int32 index tensor on the cache's device."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or not t.is_contiguous():
         _i32(t, name)
     if t.device != dev:
         raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
@@ -215,13 +215,9 @@ def _ids(t: torch.Tensor, name: str, dev: torch.device) -> int:
 
 def _rows(t: torch.Tensor, name: str, shape: tuple, dt: torch.dtype, dev: torch.device) -> tuple:
     """Strides of [n, heads, head_dim] rows, whose type, shape and place are checked."""
-    if t.dtype != dt:
-        raise ValueError(f"{name} must be {dt}, not {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {list(shape)}")
     st = t.stride()
-    if st[2] != 1:
-        raise ValueError(f"{name} must have a unit inner stride")
+    if t.dtype is not dt or t.shape != shape or st[2] != 1:
+        raise ValueError(f"{name} must be {list(shape)} in {dt} with a unit inner stride")
     if t.device != dev:
         raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
     return st
@@ -230,41 +226,43 @@ def _rows(t: torch.Tensor, name: str, shape: tuple, dt: torch.dtype, dev: torch.
 _ROW_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
-def _row_dtype(t: torch.Tensor, cv: CacheView) -> torch.dtype:
+def _row_dtype(t: torch.Tensor, d: int) -> torch.dtype:
     dt = t.dtype
     if dt not in _ROW_DTYPES:
         raise ValueError(f"rows must be float16, bfloat16 or float32, not {dt}")
-    if cv.head_dim % 16 or not 0 < cv.head_dim <= 512:
+    if d % 16 or not 0 < d <= 512:
         raise ValueError("head_dim must be a multiple of 16, up to 512")
     return dt
 
 
-def _append_fp8(append_key, append_value, cv, sv, err_count, batch_indices=None, positions=None, kv_indices=None,
-                kv_indptr=None, slots=None) -> None:
+def _append_fp8(append_key, append_value, paged_kv_cache, kv_layout, kv_scales, err_count, batch_indices=None, positions=None,
+                kv_indices=None, kv_indptr=None, slots=None) -> None:
     """The append into an 8-bit cache, by page table or slots."""
-    dev, dt = cv.device, _row_dtype(append_key, cv)
+    kp, vp, page_stride, pages, ps, hkv, d, cdt, dev = cache_fields(paged_kv_cache, kv_layout)
+    scales = scale_fields(kv_scales, pages, ps, hkv, cdt, dev)
+    dt = _row_dtype(append_key, d)
     nnz = append_key.shape[0]
-    shape = (nnz, cv.num_kv_heads, cv.head_dim)
+    shape = (nnz, hkv, d)
     ks, vs = _rows(append_key, "append_key", shape, dt, dev), _rows(append_value, "append_value", shape, dt, dev)
+    bi = po = sl = idx = nidx = ptr = batch = err = 0
     if slots is not None:
-        table = (0, 0, _ids(slots, "slots", dev))
+        sl = _ids(slots, "slots", dev)
         if slots.numel() < nnz:
             raise ValueError("append_key, append_value and slots disagree on nnz")
-        idx, nidx, ptr, batch = 0, 0, 0, 0
     else:
-        table = (_ids(batch_indices, "batch_indices", dev), _ids(positions, "positions", dev), 0)
+        bi, po = _ids(batch_indices, "batch_indices", dev), _ids(positions, "positions", dev)
         if batch_indices.numel() < nnz or positions.numel() < nnz:
             raise ValueError("append_key, append_value, batch_indices and positions disagree on nnz")
         idx, nidx = _ids(kv_indices, "kv_indices", dev), kv_indices.numel()
         ptr, batch = _ids(kv_indptr, "kv_indptr", dev), kv_indptr.numel() - 1
         if batch < 0:
             raise ValueError("kv_indptr must have batch+1 entries")
-    err_ptr = _i32(err_count, "err_count").data_ptr() if err_count is not None else 0
+    if err_count is not None:
+        err = _ids(err_count, "err_count", dev)
     if nnz == 0:
         return
-    check(call(CALL_APPEND_FP8, append_key.data_ptr(), ks[0], ks[1], append_value.data_ptr(), vs[0], vs[1], *table, nnz,
-               cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages, sv.k_ptr, sv.v_ptr, sv.page_stride, idx, nidx, ptr, batch,
-               cv.num_kv_heads, cv.head_dim, cv.page_size, DTYPE_CODE[dt], err_ptr, stream_ptr(dev)),
+    check(call(CALL_APPEND_FP8, append_key.data_ptr(), ks[0], ks[1], append_value.data_ptr(), vs[0], vs[1], bi, po, sl, nnz,
+               kp, vp, page_stride, pages, *scales, idx, nidx, ptr, batch, hkv, d, ps, DTYPE_CODE[dt], err, stream_ptr(dev)),
           "append_paged_kv_cache (8-bit cache)")
 
 
@@ -279,9 +277,11 @@ def append_paged_kv_cache_slots(append_key: torch.Tensor, append_value: torch.Te
     counted in ``err_count``.  With an 8-bit cache and its ``kv_scales`` the rows are quantised as
     ``append_paged_kv_cache`` does it.
     """
+    if kv_scales is not None:
+        return _append_fp8(append_key, append_value, paged_kv_cache, kv_layout, kv_scales, err_count, slots=slots)
     cv = CacheView(paged_kv_cache, kv_layout)
-    if cv.dtype == FP8 or kv_scales is not None:
-        return _append_fp8(append_key, append_value, cv, ScaleView(kv_scales, cv), err_count, slots=slots)
+    if cv.dtype is FP8:
+        raise ValueError("a float8_e4m3fn cache needs kv_scales")
     for t, n in ((append_key, "append_key"), (append_value, "append_value")):
         if t.dtype != cv.dtype:
             raise ValueError(f"{n} dtype {t.dtype} differs from the cache dtype {cv.dtype}")
@@ -392,45 +392,36 @@ def append_paged_kv_cache_with_norm_rope(q: torch.Tensor, append_key: torch.Tens
     head_dim must be a multiple of 16, up to 512.  Tokens with bad metadata are skipped, but for their
     queries, and counted in ``err_count``.
     """
-    cv = CacheView(paged_kv_cache, kv_layout)
-    sv = ScaleView(kv_scales, cv) if cv.dtype == FP8 or kv_scales is not None else None
-    dev, dt, d = cv.device, _row_dtype(append_key, cv), cv.head_dim
-    if sv is None and dt != cv.dtype:
-        raise ValueError(f"append_key dtype {dt} differs from the cache dtype {cv.dtype}")
+    kp, vp, page_stride, pages, ps, hkv, d, cache_dt, dev = cache_fields(paged_kv_cache, kv_layout)
+    dt = _row_dtype(append_key, d)
+    if kv_scales is not None or cache_dt is FP8:
+        scales = scale_fields(kv_scales, pages, ps, hkv, cache_dt, dev)
+    elif dt is cache_dt:
+        scales = _NO_SCALES
+    else:
+        raise ValueError(f"append_key dtype {dt} differs from the cache dtype {cache_dt}")
     nnz = append_key.shape[0]
-    shape = (nnz, cv.num_kv_heads, d)
+    shape = (nnz, hkv, d)
     ks, vs = _rows(append_key, "append_key", shape, dt, dev), _rows(append_value, "append_value", shape, dt, dev)
     qshape = q.shape
     if len(qshape) != 3 or qshape[0] != nnz or qshape[2] != d:
         raise ValueError(f"q must be [{nnz}, Hq, {d}] in {dt}")
     qs = _rows(q, "q", qshape, dt, dev)
-    if q_out is None:
-        q_out = torch.empty_like(q) if q.is_contiguous() else torch.empty(qshape, dtype=dt, device=dev)
-        os = q_out.stride()
-    else:
-        os = _rows(q_out, "q_out", qshape, dt, dev)
-    qw = kw = 0
-    wdt = None
-    for t, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or t.shape != (d,) or t.stride(0) != 1 or t.dtype not in (dt, torch.float32):
-            raise ValueError(f"{n} must be [{d}] in {dt} or float32 with a unit inner stride")
-        if wdt is not None and t.dtype != wdt:
+    qw = kw = err = 0
+    wdt = dt
+    if q_weight is not None:
+        qw, wdt = _weight(q_weight, "q_weight", d, dt, dev), q_weight.dtype
+    if k_weight is not None:
+        kw = _weight(k_weight, "k_weight", d, dt, dev)
+        if qw and k_weight.dtype is not wdt:
             raise ValueError("q_weight and k_weight must share one dtype")
-        if t.device != dev:
-            raise ValueError(f"{n} is on {t.device}, the cache on {dev}")
-        wdt = t.dtype
-        if n == "q_weight":
-            qw = t.data_ptr()
-        else:
-            kw = t.data_ptr()
-    cdt, cst = cos.dtype, cos.stride()
-    for t, n in ((cos, "cos"), (sin, "sin")):
-        if t.shape != (nnz, d) or (nnz and t.stride() != cst) or cst[-1] != 1 or t.dtype != cdt or cdt not in (dt, torch.float32):
-            raise ValueError(f"cos and sin must both be [{nnz}, {d}] in {dt} or float32, with one row stride and a unit inner one")
-        if t.device != dev:
-            raise ValueError(f"{n} is on {t.device}, the cache on {dev}")
+        wdt = k_weight.dtype
+    cdt, cst, cs_shape = cos.dtype, cos.stride(), cos.shape
+    if cs_shape != (nnz, d) or sin.shape != cs_shape or sin.stride() != cst or cst[1] != 1 or sin.dtype is not cdt or \
+            (cdt is not dt and cdt is not torch.float32):
+        raise ValueError(f"cos and sin must both be [{nnz}, {d}] in {dt} or float32, with one row stride and a unit inner one")
+    if cos.device != dev or sin.device != dev:
+        raise ValueError(f"cos and sin are on {cos.device} and {sin.device}, the cache on {dev}")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
     bi, po = _ids(batch_indices, "batch_indices", dev), _ids(positions, "positions", dev)
@@ -439,17 +430,32 @@ def append_paged_kv_cache_with_norm_rope(q: torch.Tensor, append_key: torch.Tens
     idx, ptr, batch = _ids(kv_indices, "kv_indices", dev), _ids(kv_indptr, "kv_indptr", dev), kv_indptr.numel() - 1
     if batch < 0:
         raise ValueError("kv_indptr must have batch+1 entries")
-    err_ptr = _i32(err_count, "err_count").data_ptr() if err_count is not None else 0
+    if err_count is not None:
+        err = _ids(err_count, "err_count", dev)
+    if q_out is None:
+        q_out = torch.empty_like(q) if q.is_contiguous() else torch.empty(qshape, dtype=dt, device=dev)
+        os = q_out.stride()
+    else:
+        os = _rows(q_out, "q_out", qshape, dt, dev)
     if nnz == 0:
         return q_out
     code = DTYPE_CODE[dt]
-    scales = (sv.k_ptr, sv.v_ptr, sv.page_stride) if sv is not None else (0, 0, 0)
     check(call(CALL_NORM_ROPE, q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), os[0], os[1], qshape[1], append_key.data_ptr(),
-               ks[0], ks[1], append_value.data_ptr(), vs[0], vs[1], qw, kw, code if wdt is None else DTYPE_CODE[wdt], float(eps),
-               cos.data_ptr(), sin.data_ptr(), cst[0], DTYPE_CODE[cdt], bi, po, nnz, cv.k_ptr, cv.v_ptr, cv.page_stride,
-               cv.num_pages, *scales, idx, kv_indices.numel(), ptr, batch, cv.num_kv_heads, d, cv.page_size, code, err_ptr,
-               stream_ptr(dev)), "append_paged_kv_cache_with_norm_rope")
+               ks[0], ks[1], append_value.data_ptr(), vs[0], vs[1], qw, kw, DTYPE_CODE[wdt], eps, cos.data_ptr(), sin.data_ptr(),
+               cst[0], DTYPE_CODE[cdt], bi, po, nnz, kp, vp, page_stride, pages, *scales, idx, kv_indices.numel(), ptr, batch,
+               hkv, d, ps, code, err, stream_ptr(dev)), "append_paged_kv_cache_with_norm_rope")
     return q_out
+
+
+_NO_SCALES = (0, 0, 0)
+
+
+def _weight(t, name: str, d: int, dt: torch.dtype, dev: torch.device) -> int:
+    if not isinstance(t, torch.Tensor) or t.shape != (d,) or not t.is_contiguous() or (t.dtype is not dt and t.dtype is not torch.float32):
+        raise ValueError(f"{name} must be [{d}] in {dt} or float32, contiguous")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
+    return t.data_ptr()
 
 
 def read_paged_kv_cache(paged_kv_cache: CacheT, kv_scales, kv_indices: torch.Tensor, kv_indptr: torch.Tensor,
@@ -461,9 +467,8 @@ def read_paged_kv_cache(paged_kv_cache: CacheT, kv_scales, kv_indices: torch.Ten
     read, with the slots past a sequence's end; an id outside the pool gives zeros; pages of ``out`` past
     the list are left as they were.  head_dim must be a multiple of 16, up to 512.
     """
-    cv = CacheView(paged_kv_cache, kv_layout)
-    sv = ScaleView(kv_scales, cv)
-    dev, d = cv.device, cv.head_dim
+    kp, vp, page_stride, pages, ps, hkv, d, cache_dt, dev = cache_fields(paged_kv_cache, kv_layout)
+    scales = scale_fields(kv_scales, pages, ps, hkv, cache_dt, dev)
     if d % 16 or not 0 < d <= 512:
         raise ValueError("head_dim must be a multiple of 16, up to 512")
     idx, ptr, batch = _ids(kv_indices, "kv_indices", dev), _ids(kv_indptr, "kv_indptr", dev), kv_indptr.numel() - 1
@@ -471,13 +476,13 @@ def read_paged_kv_cache(paged_kv_cache: CacheT, kv_scales, kv_indices: torch.Ten
         raise ValueError("kv_indptr must have batch+1 entries")
     code = dtype_code(dtype)
     n = kv_indices.numel()
-    shape = (n, 2, cv.page_size, cv.num_kv_heads, d)
+    shape = (n, 2, ps, hkv, d)
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=dev)
     elif out.shape != shape or out.dtype != dtype or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"out must be {list(shape)} in {dtype}, contiguous, on the cache's device")
     if n == 0 or batch == 0:
         return out
-    check(call(CALL_READ_FP8, cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages, sv.k_ptr, sv.v_ptr, sv.page_stride, idx, n, ptr,
-               batch, cv.num_kv_heads, d, cv.page_size, out.data_ptr(), code, stream_ptr(dev)), "read_paged_kv_cache")
+    check(call(CALL_READ_FP8, kp, vp, page_stride, pages, *scales, idx, n, ptr, batch, hkv, d, ps, out.data_ptr(), code,
+               stream_ptr(dev)), "read_paged_kv_cache")
     return out

@@ -25,7 +25,7 @@ import numpy as np
 import torch
 
 from ._lib import CALL_DECODE_FP8, DTYPE_CODE, call, check, dtype_code, lib, stream_ptr
-from .ops import FP8, CacheView, ScaleView, _i32, read_paged_kv_cache
+from .ops import FP8, CacheView, _i32, cache_fields, read_paged_kv_cache, scale_fields
 
 _STR_DTYPES = {"float8_e4m3fn": FP8, "float16": torch.float16, "half": torch.float16, "bfloat16": torch.bfloat16,
                "float32": torch.float32, "float": torch.float32}
@@ -241,31 +241,31 @@ class BatchDecodeWithPagedKVCacheWrapper:
         self._planned = True
 
     def _run_fp8(self, q: torch.Tensor, paged_kv_cache, kv_scales, out: torch.Tensor | None) -> torch.Tensor:
-        cv = CacheView(paged_kv_cache, self._kv_layout)
-        dt, qs, ws = self._q_dtype, q.stride(), self._workspace
-        if q.dtype != dt or cv.dtype != FP8:
+        kp, vp, page_stride, pages, ps, hkv, d, cache_dt, dev = cache_fields(paged_kv_cache)
+        dt, qs, shape, ws = self._q_dtype, q.stride(), q.shape, self._workspace
+        if q.dtype is not dt or cache_dt is not FP8:
             raise ValueError(f"q dtype must be {dt}, cache dtype {FP8}")
-        if q.shape != (self._batch, self._hq, self._d) or qs[2] != 1:
+        if shape != (self._batch, self._hq, self._d) or qs[2] != 1:
             raise ValueError(f"q must be [{self._batch}, {self._hq}, {self._d}] with unit inner stride")
-        if (cv.num_kv_heads, cv.head_dim, cv.page_size) != (self._hkv, self._d, self._ps):
+        if hkv != self._hkv or d != self._d or ps != self._ps:
             raise ValueError("cache geometry differs from plan()")
-        sv = ScaleView(kv_scales, cv)
-        if q.device != cv.device:
-            raise ValueError(f"q is on {q.device}, the cache on {cv.device}")
+        scales = scale_fields(kv_scales, pages, ps, hkv, cache_dt, dev)
+        if q.device != dev:
+            raise ValueError(f"q is on {q.device}, the cache on {dev}")
         if out is None:
-            out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=cv.device)
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dt, device=dev)
             st = out.stride()
         else:
             st = out.stride()
-            if out.shape != q.shape or out.dtype != dt or st[2] != 1 or out.device != cv.device:
+            if out.shape != shape or out.dtype != dt or st[2] != 1 or out.device != dev:
                 raise ValueError("out must match q's shape, dtype and device")
         qp = q.data_ptr()
         if (qp | qs[0] * 2 | qs[1] * 2) % 16:  # (rows are read 16 bytes at a time)
             q = q.clone(memory_format=torch.contiguous_format)
             qp, qs = q.data_ptr(), q.stride()
-        check(call(CALL_DECODE_FP8, qp, qs[0], qs[1], cv.k_ptr, cv.v_ptr, cv.page_stride, cv.num_pages, sv.k_ptr, sv.v_ptr,
-                   sv.page_stride, *self._args, ws.data_ptr(), ws.numel() * ws.element_size(), out.data_ptr(), st[0], st[1],
-                   DTYPE_CODE[dt], self._flags, stream_ptr(cv.device)), "BatchDecodeWithPagedKVCacheWrapper.run")
+        check(call(CALL_DECODE_FP8, qp, qs[0], qs[1], kp, vp, page_stride, pages, *scales, *self._args, ws.data_ptr(),
+                   ws.numel() * ws.element_size(), out.data_ptr(), st[0], st[1], DTYPE_CODE[dt], self._flags, stream_ptr(dev)),
+              "BatchDecodeWithPagedKVCacheWrapper.run")
         return out
 
     def run(self, q: torch.Tensor, paged_kv_cache, *args, q_scale=None, k_scale=None,
@@ -276,7 +276,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
         [batch, num_kv_heads, head_dim] with unit inner stride, first appends token b's rows at
         position seq_len_b - 1 (the decode step's append through the CUDA-graph metadata,
         ecahlang/manager.py:270-280) -- in the same launch on the matrix-core path.  ``kv_scales``: the
-        scales of a float8_e4m3fn cache (``ops.ScaleView``)."""
+        scales of a float8_e4m3fn cache (``ops.new_kv_scales``)."""
         if not self._planned:
             raise RuntimeError("plan() must be called before run()")
         if self._fp8:
