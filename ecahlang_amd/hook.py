@@ -14,7 +14,9 @@ cache (:68); advance the manager's layer counter (:89).  In the bucketed decode 
 wrapper planned on the bucket's buffers as main.py plans it, the append rides in the decode's
 launch (``run(..., append_kv=)``: the same bytes land in the same slots).  Inputs in another dtype than the
 cache (an fp32 model over an fp16 cache) are cast to the cache's dtype and the output cast
-back (the reference's ``need_autocast``, :50-53, :95-96).  ``attention_mask``, ``dropout``,
+back (the reference's ``need_autocast``, :50-53, :95-96).  Over an 8-bit cache (the manager's
+``kv_dtype``, which the wrapper is planned for too) each layer's append quantises and the wrapper gets the
+layer's scales.  ``attention_mask``, ``dropout``,
 ``scaling`` and ``sliding_window`` are ignored as in the reference: the wrapper's plan holds
 the causal structure and the 1/sqrt(head_dim) scale.  The reference's optional SDPA
 cross-check (:70-87) is a debugging aid and is not reproduced.
@@ -42,16 +44,18 @@ def ecah_attention(module, query, key, value, attention_mask, **kwargs):
     v = value[0].transpose(0, 1)
     layer_attr = "prefill_layer_idx" if prefill else "decode_layer_idx"
     layer_idx = getattr(manager, layer_attr)
+    scales = getattr(manager, "kv_scales", None)  # (an 8-bit cache's; its decode takes no append along)
+    more = {} if scales is None else {"kv_scales": scales[layer_idx]}
     if manager.cuda_graph_mode and not prefill:
-        if _planned_on_bucket(wrapper, manager, q.shape[0]):
+        if scales is None and _planned_on_bucket(wrapper, manager, q.shape[0]):
             # the bucket's append (positions = seq_len - 1) in the decode's own launch
             o = wrapper.run(q, manager.kv_cache[layer_idx], append_kv=(k, v))
         else:
             manager.append_paged_kv_cache_cuda_graph(k, v, q.shape[0], layer_idx)
-            o = wrapper.run(q, manager.kv_cache[layer_idx])
+            o = wrapper.run(q, manager.kv_cache[layer_idx], **more)
     else:
         manager.append_paged_kv_cache_cached(k, v, layer_idx)
-        o = wrapper.run(q, manager.kv_cache[layer_idx])
+        o = wrapper.run(q, manager.kv_cache[layer_idx], **more)
     setattr(manager, layer_attr, layer_idx + 1)
     o = o[None]
     if o.dtype != in_dtype:

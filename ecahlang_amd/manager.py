@@ -64,8 +64,9 @@ import numpy as np
 import torch
 
 from ._lib import check, lib, stream_ptr
-from .ops import (append_paged_kv_cache, append_paged_kv_cache_slots, get_batch_indices_positions,
-                  get_seq_lens)
+from .ops import (FP8, append_paged_kv_cache, append_paged_kv_cache_slots, get_batch_indices_positions,
+                  get_seq_lens, new_kv_scales)
+from .wrappers import _as_dtype
 
 _POP, _PUSH, _COPY, _COW = 0, 1, 2, 3
 
@@ -205,12 +206,14 @@ class AutoKVCacheManager:
                  seq_lens: int = 128, block_size: int = 16, dtype: torch.dtype = torch.float16,
                  layout: str = "NHD", total_gpu_mem_bytes: int | None = None,
                  mem_utilization: float = 0.9, *, device=None, max_pages_per_seq: int = 512,
-                 strict_reference_q1: bool = False, prefix_cache_rows: int = 0):
+                 strict_reference_q1: bool = False, prefix_cache_rows: int = 0, kv_dtype=None):
         """manager.py:14-72.  Extensions (keyword-only): ``device`` (default: the current
         CUDA device), ``max_pages_per_seq`` (initial width of the per-sequence page table; it
         grows on demand), ``strict_reference_q1`` (see the module docstring) and
         ``prefix_cache_rows`` (0: no prefix cache; otherwise how many inserts the cache keeps
-        at once, each in a row of the page table)."""
+        at once, each in a row of the page table) and
+        ``kv_dtype`` (``torch.float8_e4m3fn``: an 8-bit cache with its scales in ``kv_scales``, which the
+        appends quantise into; ``dtype`` stays that of queries, keys and values)."""
         if layout.upper() != "NHD":
             raise NotImplementedError("only the NHD cache layout is implemented (the reference uses NHD)")
         self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
@@ -235,12 +238,22 @@ class AutoKVCacheManager:
 
         if total_gpu_mem_bytes is None:
             total_gpu_mem_bytes = get_total_free_memory(self.device.index or 0)
+        self.kv_dtype = _as_dtype(kv_dtype) if kv_dtype is not None else dtype
+        if self.kv_dtype != dtype:
+            if self.kv_dtype != FP8 or head_dim % 16 or head_dim > 512 or num_kv_heads * block_size % 8:
+                raise ValueError("kv_dtype must be float8_e4m3fn (or dtype), with head_dim a multiple of 16 up to 512 "
+                                 "and num_kv_heads * block_size a multiple of 8")
         usable_mem = int(total_gpu_mem_bytes * mem_utilization)
-        per_token_bytes = num_kv_heads * head_dim * self.dtype_size * 2
+        per_row_bytes = head_dim + 1 if self.kv_dtype == FP8 else head_dim * self.dtype_size
+        per_token_bytes = num_kv_heads * per_row_bytes * 2
         per_block_per_layer = block_size * per_token_bytes
         self.max_blocks = usable_mem // (num_layers * per_block_per_layer)
         self.kv_cache = torch.zeros((num_layers, self.max_blocks, 2, block_size, num_kv_heads, head_dim),
-                                    dtype=dtype, device=self.device)
+                                    dtype=torch.uint8 if self.kv_dtype == FP8 else dtype, device=self.device)
+        self.kv_scales = None
+        if self.kv_dtype == FP8:
+            self.kv_cache = self.kv_cache.view(FP8)
+            self.kv_scales = new_kv_scales(self.kv_cache)
 
         # device pool: free-page stack (bottom = page 0) and one page-list row per sequence
         # slot, then a row for the CUDA-graph padding pages, then the prefix cache's rows
@@ -362,11 +375,11 @@ class AutoKVCacheManager:
             self._reset_mask_rows(ops, off)
         self._ops = []
         if self._n_cow:
-            c = self.kv_cache
-            check(lib().pkv_pool_copy_pages(c.data_ptr(), c.stride(0) * c.element_size(), c.shape[0],
-                                            c.stride(1) * c.element_size(), self._pairs.data_ptr(), self._n_cow,
-                                            self.max_blocks, self._err.data_ptr(), stream_ptr(self.device)),
-                  "page copy")
+            for c in (self.kv_cache,) if self.kv_scales is None else (self.kv_cache, self.kv_scales):
+                check(lib().pkv_pool_copy_pages(c.data_ptr(), c.stride(0) * c.element_size(), c.shape[0],
+                                                c.stride(1) * c.element_size(), self._pairs.data_ptr(), self._n_cow,
+                                                self.max_blocks, self._err.data_ptr() if c is self.kv_cache else 0,
+                                                stream_ptr(self.device)), "page copy")
             self._n_cow = 0
 
     # ------------------------------------------------------------------ page handles (sharing)
@@ -780,7 +793,12 @@ class AutoKVCacheManager:
                               batch_indices=self._cached_batch_indices, positions=self._cached_positions,
                               paged_kv_cache=self.kv_cache[layer_idx], kv_indices=self._cached_kv_indices,
                               kv_indptr=self._cached_kv_indptr,
-                              kv_last_page_len=self._cached_kv_last_page_len, kv_layout=self.layout)
+                              kv_last_page_len=self._cached_kv_last_page_len, kv_layout=self.layout,
+                              kv_scales=self.layer_scales(layer_idx))
+
+    def layer_scales(self, layer_idx: int):
+        """One layer's scales of an 8-bit cache, or None."""
+        return None if self.kv_scales is None else self.kv_scales[layer_idx]
 
     def append_paged_kv_cache(self, batch_ids, key, value, append_indptr, layer_idx: int, nnz=None) -> None:
         """manager.py:167-185 (the uncached variant)."""
@@ -791,7 +809,8 @@ class AutoKVCacheManager:
         append_paged_kv_cache(append_key=key, append_value=value, batch_indices=batch_indices,
                               positions=positions, paged_kv_cache=self.kv_cache[layer_idx],
                               kv_indices=kv_indices, kv_indptr=kv_indptr,
-                              kv_last_page_len=kv_last_page_len, kv_layout=self.layout)
+                              kv_last_page_len=kv_last_page_len, kv_layout=self.layout,
+                              kv_scales=self.layer_scales(layer_idx))
 
     # ------------------------------------------------------------------ CUDA-graph buckets (A10-A12)
 
@@ -858,7 +877,7 @@ class AutoKVCacheManager:
         ``kv_indices``) is resolved once per step by ``fill_cuda_graph_metadata``, so every
         layer's append reads one slot per token."""
         append_paged_kv_cache_slots(key, value, self._cg_slots[bucket_size], self.kv_cache[layer_idx],
-                                    kv_layout=self.layout)
+                                    kv_layout=self.layout, kv_scales=self.layer_scales(layer_idx))
 
     # ------------------------------------------------------------------ device-resident decode steps
 
