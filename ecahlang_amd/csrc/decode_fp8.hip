@@ -71,6 +71,16 @@ __device__ __forceinline__ int length_of(int i0, int i1, int last, int ps, int64
   return (int)min((np - 1) * ps + min(max(last, 0), ps), max(av, (int64_t)0) * ps);
 }
 __device__ __forceinline__ int tiles_of(int len) { return (len + 15) / 16; }
+// Inclusive sum over the wave's lanes, in registers: within rows of 16 lanes by row shifts, then the rows' totals.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast 31 into rows 2 and 3
+  return x;
+}
 // Parts of a sequence: of `aim` tiles at most, one if there are few.
 __device__ __forceinline__ int parts_of(int tiles, int aim, int max_parts) {
   return tiles <= max(kWholeTiles, aim) ? 1 : min((tiles + aim - 1) / aim, max_parts);
@@ -123,9 +133,11 @@ __global__ __launch_bounds__(W * 64, HB * D == 256 ? 2 : 4) void decode_fp8_kern
   // follow each other in sequence order; those and cut sequences look for their place among the batch, 64
   // sequences a round.
   typedef __attribute__((address_space(1))) uint16_t g16;  // (stores through a generic pointer would drain the loads in flight)
-  int b = min(w, B - 1), nparts, part = 0, more0 = 0;
-  int s0 = P.indptr[b], aim;
-  int len = length_of(s0, P.indptr[b + 1], P.last[b], ps, P.num_indices);
+  int b = min(w, B - 1), nparts, part = 0, more0 = 0, aim;
+  // (everything that may be needed is requested at once: my sequence's, and the first 64 sequences' for the search)
+  int i0 = P.indptr[min(lane, B)], i1 = P.indptr[min(lane + 1, B)], lv = P.last[min(lane, B - 1)];
+  int s0 = P.indptr[b];
+  const int e0 = P.indptr[b + 1], l0 = P.last[b];
   if (F.plan) {  // (made for other lengths, it may hold too few parts: the last ones are longer then)
     aim = max(F.plan[0], 1);
     nr = min(max(F.plan[1], 0), nr);
@@ -134,22 +146,18 @@ __global__ __launch_bounds__(W * 64, HB * D == 256 ? 2 : 4) void decode_fp8_kern
     const int64_t listed = max(min((int64_t)P.indptr[B], P.num_indices), (int64_t)0);
     aim = max(kMinTiles, (int)((listed * ps / 16 + nr) / nr));
   }
+  int len = length_of(s0, e0, l0, ps, P.num_indices);
   nparts = parts_of(tiles_of(len), aim, kMaxParts);
   if (w >= B || nparts > 1) {
     bool found = false;
     int base = 0;
 #pragma unroll 1
     for (int b0 = 0; b0 < B; b0 += 64) {
-      const int bl = b0 + lane, i0 = P.indptr[min(bl, B)];
-      const int ln = bl < B ? length_of(i0, P.indptr[min(bl + 1, B)], P.last[min(bl, B - 1)], ps, P.num_indices) : 0;
-      const int np = bl < B ? parts_of(tiles_of(ln), aim, kMaxParts) - 1 : 0;
-      int incl = np;
-#pragma unroll
-      for (int x = 1; x < 64; x <<= 1) {
-        const int v = __shfl_up(incl, x, 64);
-        incl += lane >= x ? v : 0;
-      }
-      const int all = __builtin_amdgcn_readlane(incl, 63);
+      const int n0 = P.indptr[min(b0 + 64 + lane, B)], n1 = P.indptr[min(b0 + 65 + lane, B)];  // (the next round's)
+      const int nl = P.last[min(b0 + 64 + lane, B - 1)];
+      const int ln = b0 + lane < B ? length_of(i0, i1, lv, ps, P.num_indices) : 0;
+      const int np = b0 + lane < B ? parts_of(tiles_of(ln), aim, kMaxParts) - 1 : 0;
+      const int incl = wave_scan(np), all = __builtin_amdgcn_readlane(incl, 63);
       if (w < B ? w < b0 + 64 : w - B < base + all) {
         const int l = w < B ? w - b0 : __popcll(__ballot(base + incl <= w - B));
         more0 = base + __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(np, l);
@@ -164,6 +172,7 @@ __global__ __launch_bounds__(W * 64, HB * D == 256 ? 2 : 4) void decode_fp8_kern
         break;
       }
       base += all;
+      i0 = n0, i1 = n1, lv = nl;
     }
     if (!found) return;  // (the grid is sized for the most parts there can be)
     nparts = 1 + min(nparts - 1, max(nr - more0, 0));  // (a kv_indptr that runs backwards)
@@ -425,7 +434,7 @@ __global__ __launch_bounds__(W * 64, HB * D == 256 ? 2 : 4) void decode_fp8_kern
     }
     top = max_across_groups(top);
     if (lg == 0) s_ml[wave][lr].x = top;
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int x = 0; x < W; ++x) top = fmaxf(top, s_ml[x][c].x);
     const float mn = top == -INFINITY ? 0.f : top;
@@ -437,7 +446,7 @@ __global__ __launch_bounds__(W * 64, HB * D == 256 ? 2 : 4) void decode_fp8_kern
     }
     sum = sum_across_groups(sum);
     if (lg == 0) s_ml[wave][lr].y = sum;
-    __syncthreads();
+    lds_barrier();
   }
   // Then the rows: four dims of one head a lane, the parts shared by nw waves; a head's partial rows are whole lines
   // of its own, so plain loads may bring them in, all of them in flight at once.
@@ -460,7 +469,7 @@ __global__ __launch_bounds__(W * 64, HB * D == 256 ? 2 : 4) void decode_fp8_kern
     }
     if (nw > 1) {
       s_x[wave * 64 + lane] = acc;
-      __syncthreads();
+      lds_barrier();
       if (sub == 0)
         for (int x = 1; x < nw; ++x) acc += s_x[(wave + x) * 64 + lane];
     }
