@@ -563,7 +563,10 @@ struct Fp8Layout {
 //    tokens 17.1 us for 15.9, of 2000 11.9 for 9.1, so heads of 128 dims take it from 128 sequences x KV heads on.
 //    Rows of two heads of 64 dims are one line of 128 bytes: always (85 sequences, 16 / 16 heads: 23 us for 35).
 //  * Eight waves a workgroup for long sequences and one-head blocks: fewer parts for as many loads in flight (one
-//    sequence of 100,003 tokens, 28 / 4 heads: 27.3 us for 33; of 2000 tokens, 16 / 2: 10.3 for 9.1).
+//    sequence of 100,003 tokens, 28 / 4 heads: 27.3 us for 33; of 2000 tokens, 16 / 2: 10.3 for 9.1; pages that are not
+//    whole tiles wait for more: 9 sequences of 100 to 9000 tokens, 32 / 8 heads, pages of 8: 16.5 for 20.4).  For
+//    two-head blocks where a CU has few tiles: half as many turns a wave (64 sequences of 512 to 4096 tokens, 16 / 2 heads:
+//    22.2 us for 23.2; of 9600, 28 / 4: 122 for 116).
 bool fp8_layout(int32_t batch, int32_t hq, int32_t hkv, int32_t d, int32_t ps, int32_t num_ctas, int64_t num_indices, Fp8Layout* L) {
   if (batch <= 0 || hkv <= 0 || hq <= 0 || hq % hkv || num_ctas <= 0 || ps <= 0 || num_indices < 0) return false;
   if (num_indices > (INT32_MAX - 64) / ps) return false;  // (tokens in 32 bits)
@@ -572,7 +575,8 @@ bool fp8_layout(int32_t batch, int32_t hq, int32_t hkv, int32_t d, int32_t ps, i
   L->two = ps % 16 == 0 && d <= 128 && hkv % 2 == 0 && g <= 8 && (d == 64 || (int64_t)batch * hkv >= 128);
   const int64_t blocks = L->two ? hkv / 2 : most;
   const int64_t cus = (num_ctas + 1) / 2, tiles = num_indices * ps / 16;
-  L->waves = d <= 128 && !L->two && tiles >= (ps % 16 ? 48 : 128) * (int64_t)batch ? 8 : 4;
+  const bool wide = L->two ? d == 128 && tiles * blocks < 48 * cus : d <= 128 && tiles >= (ps % 16 ? 48 : 128) * (int64_t)batch;
+  L->waves = wide ? 8 : 4;
   const int64_t nr = std::max<int64_t>(2 * cus / blocks, 1), slots = nr + batch;
   if (most * (slots + 8) > INT32_MAX) return false;
   // (partial rows are addressed with 31-bit byte offsets)
