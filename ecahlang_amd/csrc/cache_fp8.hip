@@ -119,7 +119,7 @@ extern "C" int pkv_append_paged_kv_cache_fp8(
   if (nnz < 0 || num_kv_heads <= 0 || page_size <= 0 || batch < 0 || num_indices < 0) return kBadArg;
   if (!head_dim_ok(head_dim)) return kBadHeadDim;
   if (nnz == 0) return kOk;
-  if (!k_scales || !v_scales || (!slots && (!batch_indices || !positions || !kv_indptr))) return kBadArg;
+  if (!append_key || !append_value || !k_scales || !v_scales || (num_pages > 0 && (!k_cache || !v_cache)) || (!slots && (!batch_indices || !positions || !kv_indptr))) return kBadArg;
   const int lanes = lanes_of(head_dim);
   const int64_t total = (int64_t)nnz * 2 * num_kv_heads;
   if (total > INT32_MAX) return kBadArg;
@@ -162,7 +162,7 @@ extern "C" int pkv_read_paged_kv_cache_fp8(const void* k_cache, const void* v_ca
   if (num_kv_heads <= 0 || page_size <= 0 || batch < 0 || num_indices < 0 || num_pages < 0) return kBadArg;
   if (!head_dim_ok(head_dim)) return kBadHeadDim;
   if (num_indices == 0 || batch == 0) return kOk;
-  if (!kv_indptr || !kv_indices || !out) return kBadArg;
+  if (!kv_indptr || !kv_indices || !out || (num_pages > 0 && (!k_cache || !v_cache || !k_scales || !v_scales))) return kBadArg;
   if (!page_fits(page_size, num_kv_heads, head_dim)) return kBadArg;
   if ((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)page_stride) % 8) || (uintptr_t)out % 16) return kBadAlign;
   const ReadArgs a{(const uint8_t*)k_cache, (const uint8_t*)v_cache, (const uint8_t*)k_scales, (const uint8_t*)v_scales,

@@ -306,7 +306,8 @@ __global__ __launch_bounds__(W * 64, HB * D == 256 ? 2 : 4) void decode_fp8_kern
         sj = Mma<T>::qk(a1, qr[2 * (j % (NK / HB)) + 1], sj);
       }
     }
-    float sc[4], vsf[4];
+    float sc[4];
+    int ev[4];
     if (HB == 1) sa += sb;
     else sa = hn == 0 ? sa : sb;
     if constexpr (!P16) {
@@ -323,7 +324,13 @@ __global__ __launch_bounds__(W * 64, HB * D == 256 ? 2 : 4) void decode_fp8_kern
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       sc[i] = ldexpf(sa[i], (int)((ke >> (8 * i)) & 255) - 127) * P.scale_log2;
-      vsf[i] = __uint_as_float(((ve >> (8 * i)) & 255) << 23);
+      ev[i] = (int)((ve >> (8 * i)) & 255) - 127;
+    }
+    const uint32_t both = ke | ve;
+    if (__ballot((~both - 0x01010101u) & both & 0x80808080u)) {  // a byte of 255, perhaps: NaN
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (((ke >> (8 * i)) & 255) == 255 || ev[i] == 128) sc[i] = NAN;
     }
     load_k(next);
     if (!full) {
@@ -332,7 +339,6 @@ __global__ __launch_bounds__(W * 64, HB * D == 256 ? 2 : 4) void decode_fp8_kern
       for (int i = 0; i < 4; ++i) {
         const bool x = in >> i & 1;
         sc[i] = x ? sc[i] : -INFINITY;
-        vsf[i] = x ? vsf[i] : 0.f;
 #pragma unroll
         for (int c = 0; c < VW; ++c) vr[i][c] = x ? vr[i][c] : 0u;
       }
@@ -353,7 +359,7 @@ __global__ __launch_bounds__(W * 64, HB * D == 256 ? 2 : 4) void decode_fp8_kern
     for (int i = 0; i < 4; ++i) sc[i] = __builtin_amdgcn_exp2f(sc[i] - nm);
     lsum += (sc[0] + sc[1]) + (sc[2] + sc[3]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) wt[i] = sc[i] * vsf[i];
+    for (int i = 0; i < 4; ++i) wt[i] = ldexpf(sc[i], ev[i]);
     using M16 = Mma<__hip_bfloat16>;
     const uint32_t h01 = M16::pack(wt[0], wt[1]), h23 = M16::pack(wt[2], wt[3]);
     rest[0] = wt[0] - __uint_as_float(h01 << 16), rest[1] = wt[1] - __uint_as_float(h01 & 0xFFFF0000u);
@@ -548,8 +554,10 @@ namespace {
 
 inline int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
-// Workspace: [counters: int32 a sequence and head block] [part_ml: S x ml_slot_stride(Hq) float2]
+// Workspace: [counters: int32 a sequence and head block, kCounters of them at least, so that of wrappers that take
+// turns on one workspace none lays its partials on another's] [the plan] [part_ml: S x ml_slot_stride(Hq) float2]
 // [part_o: f32 S x Hq x D], S = nr + batch partial slots.
+constexpr int64_t kCounters = 8192;
 struct Fp8Layout {
   int64_t plan, ml, o, total;
   int32_t nr;             // further parts there is room for
@@ -583,7 +591,7 @@ bool fp8_layout(int32_t batch, int32_t hq, int32_t hkv, int32_t d, int32_t ps, i
   if (slots * hq * d * (int64_t)sizeof(float) > INT32_MAX) return false;
   L->nr = (int32_t)nr;
   L->blocks = (int32_t)blocks;
-  L->plan = align256(sizeof(int32_t) * batch * most);
+  L->plan = align256(sizeof(int32_t) * std::max(batch * most, kCounters));
   L->ml = L->plan + 256;
   L->o = L->ml + align256((int64_t)sizeof(float2) * slots * ml_slot_stride(hq));
   L->total = L->o + align256((int64_t)sizeof(float) * slots * hq * d);
@@ -605,8 +613,10 @@ extern "C" int pkv_decode_fp8_plan(const int32_t* kv_indptr, int64_t num_indices
                                    int32_t page_size, int32_t num_ctas, void* workspace, int64_t workspace_bytes,
                                    void* stream) {
   Fp8Layout L;
-  if (!fp8_layout(batch, num_qo_heads, num_kv_heads, head_dim, page_size, num_ctas, num_indices, &L) || batch > kPlanSeqs)
+  if (!fp8_layout(batch, num_qo_heads, num_kv_heads, head_dim, page_size, num_ctas, num_indices, &L) || batch > kPlanSeqs ||
+      !kv_indptr || !kv_last_page_len || !workspace)
     return kBadArg;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return kBadHeadDim;
   if (L.total > workspace_bytes) return kWorkspaceTooSmall;
   const int row = (L.two ? 2 : 1) * head_dim, unit = 256 / row;  // (a tile of a 256-byte row takes 0.4 us of a CU)
   hipLaunchKernelGGL(decode_fp8_plan_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, kv_indptr, kv_last_page_len, batch,
@@ -627,7 +637,8 @@ extern "C" int pkv_batch_decode_fp8(const void* q, int64_t q_stride_n, int64_t q
   if (num_kv_heads <= 0 || num_qo_heads <= 0 || num_qo_heads % num_kv_heads) return kBadGroup;
   if (page_size <= 0) return kBadPageSize;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return kBadHeadDim;
-  if (num_pages < 0) return kBadArg;
+  if (num_pages < 0 || (num_pages > 0 && (!k_cache || !v_cache || !k_scales || !v_scales))) return kBadArg;
+  if (!q || !out || !kv_indptr || !kv_last_page_len || (num_indices > 0 && !kv_indices) || !workspace) return kBadArg;
   Fp8Layout L;
   if (!fp8_layout(batch, num_qo_heads, num_kv_heads, head_dim, page_size, num_ctas, num_indices, &L)) return kBadArg;
   if (L.total > workspace_bytes) return kWorkspaceTooSmall;
@@ -663,7 +674,7 @@ extern "C" int pkv_batch_decode_fp8(const void* q, int64_t q_stride_n, int64_t q
   else { PKV_DECODE_FP8_W(T, D, HB, P16, 4); }
 #define PKV_DECODE_FP8(T)                                                                                     \
   if (head_dim == 64) {                                                                                       \
-    if (two) { PKV_DECODE_FP8_P(T, 64, 2, true); }                                                            \
+    if (two) { PKV_DECODE_FP8_W(T, 64, 2, true, 4); }                                                         \
     else if (p16) { PKV_DECODE_FP8_P(T, 64, 1, true); }                                                       \
     else { PKV_DECODE_FP8_P(T, 64, 1, false); }                                                               \
   } else if (head_dim == 128) {                                                                               \

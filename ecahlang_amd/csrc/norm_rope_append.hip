@@ -176,6 +176,8 @@ extern "C" int pkv_append_paged_kv_cache_norm_rope(
   if (!head_dim_ok(head_dim)) return kBadHeadDim;
   if (nnz == 0) return kOk;
   const bool quant = k_scales != nullptr;
+  if (!append_key || !append_value || (num_qo_heads > 0 && (!q || !q_out)) || (num_pages > 0 && (!k_cache || !v_cache)))
+    return kBadArg;
   if (quant != (v_scales != nullptr) || !cos || !sin || !batch_indices || !positions || !kv_indptr) return kBadArg;
   const int lanes = lanes_of(head_dim), per = 64 / lanes, rows = num_qo_heads + 2 * num_kv_heads;
   const int64_t total = (int64_t)nnz * rows;

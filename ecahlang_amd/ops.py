@@ -168,7 +168,8 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor,
     With an 8-bit cache (``torch.float8_e4m3fn``) and its ``kv_scales`` (see ``new_kv_scales``) the rows, fp16,
     bf16 or fp32, are quantised as they are written: each (token, head) row gets the smallest power of
     two s >= 2^-126 with max|x| <= 448 s as its scale and is stored as the e4m3 values nearest to x / s.
-    Elements that are not finite are stored as NaN.  head_dim must be a multiple of 16, up to 512.
+    Elements that are not finite are stored as NaN.  head_dim must be a multiple of 16, up to 512.  Of two
+    tokens in one slot either's codes may meet the other's scale.
     """
     if kv_scales is not None:
         return _append_fp8(append_key, append_value, paged_kv_cache, kv_layout, kv_scales, err_count, batch_indices, positions,

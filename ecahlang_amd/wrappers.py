@@ -150,6 +150,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
         self._q_dtype = _as_dtype(q_data_type)
         self._kv_dtype = _as_dtype(kv_data_type) if kv_data_type is not None else self._q_dtype
         self._fp8 = self._kv_dtype == FP8 and self._q_dtype in (torch.float16, torch.bfloat16)
+        self._planned = False
         if self._kv_dtype != self._q_dtype and not self._fp8:
             raise NotImplementedError("q and kv must share one dtype, or be float16 / bfloat16 and float8_e4m3fn")
         self._sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(self._d)
@@ -228,9 +229,13 @@ class BatchDecodeWithPagedKVCacheWrapper:
         if need > ws.numel() * ws.element_size():
             raise RuntimeError(f"decode workspace too small: need {need} bytes")
         counters = self._batch * self._hkv * -(-self._hq // self._hkv // 16)
-        if counters > self._counters_ready:
+        # (a 16-bit wrapper on the same workspace leaves the first _MAX_HEAD_COUNTERS words alone, an 8-bit one the first
+        # _INIT_COUNTERS)
+        if counters > min(self._counters_ready, _MAX_HEAD_COUNTERS):
             check(lib().pkv_decode_workspace_init(ws.data_ptr(), counters, stream_ptr(dev)), "decode plan")
-        self._counters_ready = counters  # (the words after these are overwritten)
+            self._counters_ready = counters
+        else:
+            self._counters_ready = min(self._counters_ready, _INIT_COUNTERS)
         if self._batch <= _PLAN_SEQS and pages * self._ps * self._hkv > _PLAN_TOKENS:
             check(lib().pkv_decode_fp8_plan(
                 self._indptr.data_ptr(), pages, self._last.data_ptr(), self._batch, self._hq, self._hkv, self._d, self._ps,
@@ -408,6 +413,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         self._use_cuda_graph = use_cuda_graph
         self._planned = False
         self._list_ready = None
+        self._captured_lists = []  # page numbers that captured runs over an 8-bit cache read
 
     @property
     def is_cuda_graph_enabled(self) -> bool:
@@ -440,6 +446,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         self._q_dtype = _as_dtype(q_data_type)
         self._kv_dtype = _as_dtype(kv_data_type) if kv_data_type is not None else self._q_dtype
         self._fp8 = self._kv_dtype == FP8 and self._q_dtype in (torch.float16, torch.bfloat16)
+        self._planned = False
         if self._kv_dtype != self._q_dtype and not self._fp8:
             raise NotImplementedError("q and kv must share one dtype, or be float16 / bfloat16 and float8_e4m3fn")
         self._sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(self._d)
@@ -469,6 +476,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
             n = min(n, max(0, self._n_pages if self._mfma else int(self._indptr[-1])))
         self._read_list = self._indices[:n]
         self._indices = torch.arange(n, dtype=torch.int32, device=self._indptr.device)
+        self._read_stream = stream_ptr(self._indptr.device)
 
     # rows per matrix-core work item (8 waves x 32 rows, fp32 8 x 16): rows / g query tokens of one KV head
     _ROWS, _ROWS_F32 = 256, 128
@@ -559,6 +567,10 @@ class BatchPrefillWithPagedKVCacheWrapper:
             pages = read_paged_kv_cache(paged_kv_cache, kv_scales, self._read_list, self._indptr, self._q_dtype,
                                         kv_layout=self._kv_layout)
             cv = CacheView(pages)
+            if torch.cuda.is_current_stream_capturing():
+                self._captured_lists.append(self._indices)
+            elif stream_ptr(q.device) != self._read_stream:
+                self._indices.record_stream(torch.cuda.current_stream(q.device))
         aligned = q.data_ptr() % 16 == 0 and (q.stride(0) * q.element_size()) % 16 == 0 and \
             (q.stride(1) * q.element_size()) % 16 == 0
         mfma = self._mfma and aligned and not force_valu

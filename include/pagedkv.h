@@ -110,8 +110,9 @@ int pkv_append_paged_kv_cache_rope(const void* q, int64_t q_stride_n, int64_t q_
  * + slot], V alike (for one tensor [pages, 2, Hkv, page_size]: v_scales = k_scales + Hkv * page_size,
  * scale_page_stride = 2 * Hkv * page_size).  The writers choose the smallest power of two >= 2^-126
  * with max|x| <= 448 * scale over the row's finite elements (e = 1 .. 247) and store the e4m3 value
- * nearest to x / scale, ties to even; an element that is not finite becomes NaN.  head_dim is a
- * multiple of 16, up to 512 (the decode: 64, 128 or 256). */
+ * nearest to x / scale, ties to even; an element that is not finite becomes NaN.  Readers take any e:
+ * 0 is 2^-127, 255 NaN.  Of two tokens in one slot either's codes may meet the other's scale: give a
+ * slot once a call.  head_dim is a multiple of 16, up to 512 (the decode: 64, 128 or 256). */
 
 /* pkv_append_paged_kv_cache (slots NULL) or pkv_append_paged_kv_cache_slots (slots given:
  * batch_indices, positions, kv_indices and kv_indptr are not read) into an 8-bit cache.  `dtype` is
@@ -159,7 +160,8 @@ int pkv_read_paged_kv_cache_fp8(const void* k_cache, const void* v_cache, int64_
  * head_dim 64, 128 or 256, any page size and group, up to 2^31 - 64 tokens that num_indices pages hold.
  * The page table is read when the call runs.  The workspace (pkv_decode_fp8_workspace_bytes) starts
  * with batch * Hkv * ceil(group / 16) arrival counters, zeroed once (pkv_decode_workspace_init of
- * that many) and left at zero; it belongs to one call at a time.  q rows, the caches and page_stride
+ * that many) and left at zero; it belongs to one call at a time, and calls that take turns on it leave
+ * its first 8192 words (int32) to each other's counters.  Values above 2^119 may overflow the sums.  q rows, the caches and page_stride
  * have to be multiples of 16 bytes, for a page_size that is a multiple of 16 the scales and their
  * stride of 4.  pkv_decode_fp8_plan (optional; batch <= 4096; one small launch) writes into the
  * workspace how long a part of a sequence should be for these lengths, which calls with `flags`
