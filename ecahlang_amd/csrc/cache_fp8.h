@@ -4,8 +4,8 @@
 // mantissa bits, largest value 448, 0x7F / 0xFF NaN) and one E8M0 scale byte e, the power of two
 // 2^(e - 127): the smallest one >= 2^-126 with max|x| <= 448 * 2^(e - 127).  A power of two, and not
 // max|x| / 448, because e4m3 rounds relative to the value, so a scale up to twice as large costs no
-// precision (only values under max|x| / 2^14 come out coarser), and then x / scale is exact: the only
-// rounding is the one to e4m3, a row read back and written again comes out the same, and every stored
+// precision (only values under max|x| / 2^13 come out coarser), and then x / scale is exact: the only
+// rounding is the one to e4m3, a row read back and written again keeps its values, and every stored
 // value is exact in bfloat16.  It also takes one byte a row where fp32 takes four.  Elements that are
 // not finite are stored as NaN; the scale is that of the others.
 //
@@ -153,11 +153,11 @@ __device__ __forceinline__ float group_sum(float v, int n) {
   }));
 }
 
-// The scale byte of a row whose group of n lanes holds 16 values each (act: this lane does).
-__device__ __forceinline__ int row_scale(const float (&x)[8], const float (&y)[8], bool act, int n) {
+// The largest finite magnitude of a row whose group of n lanes holds 16 values each (act: this lane does).
+__device__ __forceinline__ uint32_t row_amax(const float (&x)[8], const float (&y)[8], bool act, int n) {
   uint32_t m = group_max(act ? amax_bits(x, y) : 0u, n);
   if (__ballot(m >= kInfBits)) m = group_max(act ? amax_bits(x, y, true) : 0u, n);
-  return scale_byte(m);
+  return m;
 }
 
 // Lanes a row of d elements takes, 16 elements each (8 of either half), rounded up to a power of two:

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) void append_fp8_kernel(AppendArgs a) {
     float x[8], y[8];
     lo.get(x);
     hi.get(y);
-    const int e = row_scale(x, y, act, a.lanes);
+    const int e = scale_byte(row_amax(x, y, act, a.lanes));
     const float inv = inv_scale(e);
     if (ok && act) {
       uint8_t* dst = (uint8_t*)(isv ? a.o.v : a.o.k) + page * a.o.page_stride + (uint32_t)((slot * hkv + h) * a.d + d0);

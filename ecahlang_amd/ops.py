@@ -389,7 +389,8 @@ def append_paged_kv_cache_with_norm_rope(q: torch.Tensor, append_key: torch.Tens
     unchanged.  ``q_weight`` / ``k_weight`` ``[head_dim]`` (``None``: rows of that kind are rotated only; both of
     one type) and ``cos`` / ``sin`` ``[nnz, head_dim]`` are in the rows' type or fp32; a weight that a model
     keeps as an offset from one is passed as ``1 + w``.  The cache is in the rows' type, or an 8-bit one with
-    its ``kv_scales``: then keys (from fp32) and values are quantised as ``append_paged_kv_cache`` does it.
+    its ``kv_scales``: then keys and values are quantised as ``append_paged_kv_cache`` does it, the keys as if
+    they had been computed exactly (where an fp32 key is next to a tie, it is computed again in 64 bits).
     head_dim must be a multiple of 16, up to 512.  Tokens with bad metadata are skipped, but for their
     queries, and counted in ``err_count``.
     """

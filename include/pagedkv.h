@@ -133,7 +133,8 @@ int pkv_append_paged_kv_cache_fp8(const void* append_key, int64_t k_stride_n, in
  * then y * cos + rotate_half(y) * sin; fp32 throughout, rounded once.  q_weight / k_weight [head_dim]
  * (NULL: rows of that kind are rotated only) have type weight_dtype, cos / sin [nnz, head_dim] type
  * cs_dtype: `dtype` or fp32.  With k_scales / v_scales the cache is an 8-bit one, else (both NULL)
- * of type `dtype`; value rows are rounded to e4m3, or copied.  q_out == q works in place.  Bad
+ * of type `dtype`; value rows are rounded to e4m3, or copied, and e4m3 keys are those nearest to the
+ * exact y (next to a tie it is computed in 64 bits).  q_out == q works in place.  Bad
  * metadata is skipped and counted once per token in *err_count (may be NULL); the token's query
  * rows are written all the same. */
 int pkv_append_paged_kv_cache_norm_rope(

@@ -131,6 +131,24 @@ def test_appends_and_reads_captured_and_replayed():
     assert err.item() == 0
 
 
+@pytest.mark.parametrize("dtype,hq,hkv,d,wdt,cdt", [
+    (torch.bfloat16, 16, 8, 128, None, None), (torch.float16, 3, 4, 64, None, None), (torch.bfloat16, 1, 4, 256, None, torch.float32),
+    (torch.float16, 2, 3, 80, torch.float32, None), (torch.float32, 4, 2, 512, None, None), (torch.bfloat16, 5, 5, 16, torch.float32, torch.float32)])
+@pytest.mark.parametrize("weights", [True, False])
+def test_quantised_keys_are_those_of_64_bits(dtype, hq, hkv, d, wdt, cdt, weights):
+    # bit for bit: next to a tie of e4m3 an fp32 key would round to the other side now and then
+    eps = 2.0 ** -17  # (the same in any type)
+    kv = [1500, 900, 7]
+    t, q, k, v, qw, kw, cos, sin = _norm_case(dtype, hq, hkv, d, 16, 21 + d, wdt=wdt, cdt=cdt, kv=kv, new=kv)
+    qw, kw = (qw, kw) if weights else (None, None)
+    codes, scales = pool8(t["pool"], 16, hkv, d)
+    cache, sc = on_dev(codes, scales)
+    ops.append_paged_kv_cache_with_norm_rope(q, k, v, qw, kw, cos, sin, dev(t["b"]), dev(t["pos"]), cache, dev(t["indices"]),
+                                             dev(t["indptr"]), dev(t["last"]), eps=eps, kv_scales=sc)
+    want = fp8_ref.norm_rotate(f64(k), f64(kw) if weights else None, f64(cos), f64(sin), eps)
+    same(cache, sc, *expected(codes, scales, t, torch.from_numpy(want), v))
+
+
 def test_two_streams_at_once():
     ps, hq, hkv, d, dtype = 16, 16, 2, 128, torch.float16
     t, q, k, v, qw, kw, cos, sin = _norm_case(dtype, hq, hkv, d, ps, 6, kv=(3000, 500, 77), new=(300, 9, 77))
