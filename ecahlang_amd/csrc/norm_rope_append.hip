@@ -54,7 +54,7 @@ struct NormRopeArgs {
 // With u = 2^-24: the sum of squares is off by at most 10 u (a chain of 4, 2 sums, up to 5 exchanges, less 1: the first
 // product is the fused one's), the mean with eps by 2, so the root by 6, its reciprocal's step by 2; factor and weight
 // 2; the rotation's product and sum 2: 12 u of |x| + |y|, a little more for cos and sin that a model scales.  The few
-// rows that hold an undecided key (1 in some 100) are computed in 64 bits; doing so for all keys takes 143 us for 84 in
+// rows that hold an undecided key (1 in some 50) are computed in 64 bits; doing so for all keys takes 143 us for 84 in
 // the bulk above, and |x c| + |y s| for each key, which flags a third fewer, 91 (its registers leave 4 waves of 5).
 constexpr float kErr = 14.f / (1 << 24);
 constexpr uint32_t kUlps = 64;  // of the largest magnitude, that picks the scale: it is at least half of its |x| + |y|
