@@ -14,11 +14,14 @@
 // the rotation's partners meet in one lane and the sum of squares takes a few lane exchanges.  The rows of all
 // tokens are dealt out in one run, 8 of 128 dims to a wave, whatever the heads of a token are: a wave that kept
 // to one token, its angles in registers, idled lanes wherever the heads do not divide by 8 and waited for each
-// token's page by itself (4003 tokens, 32 / 8 heads of 128: 20 us for 30, a step of 4 tokens 3.0 for 4.8).
+// token's page by itself (4003 tokens, 32 / 8 heads of 128: 20 us for 30, a step of 4 tokens 3.0 for 4.8).  All
+// keys come first, then all values, then all queries, so that a wave has one kind to do (token by token, waves of
+// several kinds do the work of each: 16,003 tokens into 8 bits, 14 / 2 heads of 64, 17.8 us for 23.3, 16 / 2 of 128, 40.7
+// for 43.6; where 8 divides the heads it gains nothing, and the angles are read twice: 32 / 8 of 128 into bf16 80.4 for 78.6).
 //
 // What bounds it: the bytes, beside some 250 vector instructions a wave's 8 rows, about half the time at full
 // rate: 16,003 tokens, 32 / 8 heads of 128, bf16 into 8 bits, 84.5 us for 369 MB (71 at the rate of a large
-// copy), 2 us of them to look for undecided keys and 3 for the chain of latencies of those found; into bf16 79 us (77).
+// copy), 2 us of them to look for undecided keys and 3 for the chain of latencies of those found; into bf16 80 us (77).
 #include "cache_fp8.h"
 #include "../../include/pagedkv.h"
 
@@ -45,7 +48,7 @@ struct NormRopeArgs {
   float eps;
   Table t;
   Dest o;
-  Div rows;
+  Div hqd, hkvd;
   int32_t nnz, hq, hkv, d, lanes;
   int32_t* err;
 };
@@ -157,7 +160,7 @@ __device__ __forceinline__ void exact_key(int tok, int h, int page, int slot) {
   if (lane == 0) a.o.ks[page * a.o.scale_stride + (h * a.t.ps.d + slot)] = (uint8_t)e;
 }
 
-// Rows of all tokens in one run (token, then query, key and value heads): a group of lanes takes one row at a
+// Rows of all tokens in one run (keys, values, queries; heads fastest): a group of lanes takes one row at a
 // time, wherever tokens end.  Everything a row needs is requested at once; only key and value rows look up
 // their page.
 template <typename T, typename WT, typename CT, bool QUANT, bool VEC>
@@ -165,16 +168,17 @@ __global__ __launch_bounds__(256, 4) void norm_rope_kernel(NormRopeArgs a) {
   const int lane = threadIdx.x & 63, sub = lane & (a.lanes - 1), per = 64 / a.lanes, half = a.d / 2;
   const bool act = 8 * sub < half;
   const int d0 = act ? 8 * sub : 0;
-  const uint32_t total = (uint32_t)a.nnz * a.rows.d;
+  const uint32_t keys = (uint32_t)a.nnz * a.hkv, total = 2 * keys + (uint32_t)a.nnz * a.hq;
   const uint32_t stride = gridDim.x * (blockDim.x >> 6) * per;
   const float inv_d = 1.f / (float)a.d;
   uint32_t base = __builtin_amdgcn_readfirstlane((blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6)) * per);
   for (; base < total; base += stride) {
     const uint32_t at = base + lane / a.lanes, idx = at < total ? at : total - 1;
-    const uint32_t tok = a.rows.of(idx);
-    const int row = idx - tok * a.rows.d;
-    const bool isq = row < a.hq, isv = row >= a.hq + a.hkv, in = at < total && act;
-    const int h = isq ? row : (isv ? row - a.hq - a.hkv : row - a.hq);
+    const bool isq = idx >= 2 * keys, isv = !isq && idx >= keys, in = at < total && act;
+    const uint32_t row = isq ? idx - 2 * keys : isv ? idx - keys : idx;
+    const Div heads{isq ? a.hqd.m : a.hkvd.m, isq ? a.hqd.l : a.hkvd.l, isq ? a.hqd.d : a.hkvd.d};
+    const uint32_t tok = heads.of(row);
+    const int h = row - tok * heads.d;
     const Strides st{isq ? a.qs.n : isv ? a.vs.n : a.ks.n, isq ? a.qs.h : isv ? a.vs.h : a.ks.h};
     const T* src = (const T*)row_at(isq ? a.q : isv ? a.v : a.k, st, tok, h) + d0;
     Eight<T, VEC> lo, hi;
@@ -182,16 +186,18 @@ __global__ __launch_bounds__(256, 4) void norm_rope_kernel(NormRopeArgs a) {
     hi.load(src + half);
     const CT *cosr = (const CT*)row_at(a.cos, a.cs, tok, 0) + d0, *sinr = (const CT*)row_at(a.sin, a.cs, tok, 0) + d0;
     Eight<CT, VEC> c0, c1, s0, s1;
-    c0.load(cosr);
-    c1.load(cosr + half);
-    s0.load(sinr);
-    s1.load(sinr + half);
+    if (__ballot(!isv)) {
+      c0.load(cosr);
+      c1.load(cosr + half);
+      s0.load(sinr);
+      s1.load(sinr + half);
+    }
     asm volatile("" ::: "memory");
     int page = 0, slot = 0;
     bool ok = false;
     if (!isq) {
       ok = resolve(a.t, tok, page, slot);
-      if (!ok && at < total && row == a.hq && sub == 0 && a.err) atomicAdd(a.err, 1);
+      if (!ok && at < total && !isv && h == 0 && sub == 0 && a.err) atomicAdd(a.err, 1);
     }
     float x[8], y[8];
     lo.get(x);
@@ -300,7 +306,7 @@ extern "C" int pkv_append_paged_kv_cache_norm_rope(
   const NormRopeArgs a{q, q_out, append_key, append_value, qs, os, ks, vs, q_weight, k_weight, cos, sin, cs, eps,
                        {batch_indices, positions, nullptr, kv_indices, kv_indptr, num_indices, num_pages, batch, Div(page_size)},
                        {k_cache, v_cache, (uint8_t*)k_scales, (uint8_t*)v_scales, page_stride, scale_page_stride},
-                       Div(rows), nnz, num_qo_heads, num_kv_heads, head_dim, lanes, err_count};
+                       Div(num_qo_heads ? num_qo_heads : 1), Div(num_kv_heads), nnz, num_qo_heads, num_kv_heads, head_dim, lanes, err_count};
   const uintptr_t m = (uintptr_t)q | (uintptr_t)q_out | (uintptr_t)append_key | (uintptr_t)append_value;
   const uintptr_t an = (uintptr_t)cos | (uintptr_t)sin, ws = (uintptr_t)q_weight | (uintptr_t)k_weight;
   const uintptr_t to = (uintptr_t)k_cache | (uintptr_t)v_cache;
