@@ -23,8 +23,8 @@ def test_wrappers_take_turns_on_one_workspace():
     # each lays its partials behind counters that are its own and the others' alike
     ws = workspace()
     turns = []
-    for i, (kv, hq, hkv, dtype) in enumerate([([5000, 3], 8, 2, torch.float16), ([900] * 70, 16, 8, torch.bfloat16),
-                                              ([700] * 400, 40, 8, torch.float16), ([2500, 1, 4000], 28, 4, torch.bfloat16)]):
+    for i, (kv, hq, hkv, dtype) in enumerate([([5000, 3], 8, 2, torch.float16), ([3000] + [200] * 69, 16, 8, torch.bfloat16),
+                                              ([60] * 399 + [1500], 40, 8, torch.float16), ([2500, 1, 4000], 28, 4, torch.bfloat16)]):
         t, codes, scales, q = batch(kv, 16, hq, hkv, 128, dtype, seed=i)
         w = BatchDecodeWithPagedKVCacheWrapper(ws, "NHD")
         turns.append((w, t, codes, scales, q, *on_dev(codes, scales), kv, hq, hkv, dtype))
@@ -263,3 +263,54 @@ def test_one_token_and_the_largest_heads():
         got = ops.read_paged_kv_cache(cache, sc, dev(t["indices"]), dev(t["indptr"]), torch.float32)
         vals = fp8_ref.values(*expected(codes, scales, t, k, v))[t["indices"][0]]
         np.testing.assert_array_equal(f64(got)[0, :, 0], vals[:, 0])
+
+
+@pytest.mark.parametrize("ps", [16, 8])
+def test_batches_without_a_token(ps):
+    # zero rows, and rows of a batch's empty sequences, wherever they stand
+    hq, hkv, d, dtype = 16, 2, 128, torch.float16
+    cache = torch.zeros((3, 2, ps, hkv, d), dtype=torch.uint8, device=DEV).view(F8)
+    sc = ops.new_kv_scales(cache)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    for indptr, indices, last in ((i32(0, 0, 0), i32(), i32(0, 0)), (i32(0, 0), i32(1, 2), i32(7))):
+        w = BatchDecodeWithPagedKVCacheWrapper(workspace(), "NHD")
+        w.plan(indptr, indices, last, hq, hkv, d, ps, q_data_type=dtype, kv_data_type=F8)
+        out = torch.full((last.numel(), hq, d), float("nan"), dtype=dtype, device=DEV)
+        w.run(torch.randn_like(out.float()).to(dtype), cache, kv_scales=sc, out=out)
+        assert not out.any()
+    kv = [0, 70, 0, 0, 3000, 1, 0]
+    t, codes, scales, q = batch(kv, ps, hq, hkv, d, dtype, seed=9)
+    out = planned(t, hq, hkv, d, ps, dtype).run(q, on_dev(codes, scales)[0], kv_scales=on_dev(codes, scales)[1])
+    check(out, q, t, codes, scales, kv, ps)
+
+
+def test_more_sequences_than_a_plan_looks_at():
+    kv = [1 + i % 5 for i in range(4500)]
+    kv[7], kv[4400] = 2000, 900
+    t, codes, scales, q = batch(kv, 16, 4, 2, 64, torch.bfloat16, seed=10)
+    out = planned(t, 4, 2, 64, 16, torch.bfloat16).run(q, on_dev(codes, scales)[0], kv_scales=on_dev(codes, scales)[1])
+    check(out, q, t, codes, scales, kv, 16, rows=[0, 7, 8, 4095, 4096, 4400, 4499])
+
+
+def test_pages_shared_by_sequences():
+    kv, ps, hq, hkv, d, dtype = [600, 50], 16, 16, 2, 128, torch.bfloat16
+    t, codes, scales, q = batch(kv, ps, hq, hkv, d, dtype, seed=11)
+    n = t["indptr"][1]
+    shared = dict(indptr=np.array([0, n, 2 * n, 3 * n], np.int32), indices=np.tile(t["indices"][:n], 3), last=np.array([8, 8, 1], np.int32))
+    cache, sc = on_dev(codes, scales)
+    q3 = q[[0, 0, 0]].contiguous()
+    out = planned(shared, hq, hkv, d, ps, dtype).run(q3, cache, kv_scales=sc)
+    check(out, q3, shared, codes, scales, [600, 600, 593], ps)
+    pages = ops.read_paged_kv_cache(cache, sc, dev(shared["indices"]), dev(shared["indptr"]), dtype)
+    assert torch.equal(pages[:n].view(torch.int16), pages[n:2 * n].view(torch.int16))
+
+
+def test_rotation_without_query_heads():
+    t, q, k, v, qw, kw, cos, sin = _norm_case(torch.float16, 1, 3, 64, 16, 12)
+    args = (qw, kw, cos, sin, dev(t["b"]), dev(t["pos"]))
+    tab = (dev(t["indices"]), dev(t["indptr"]), dev(t["last"]))
+    both = [torch.zeros((t["pool"], 2, 16, 3, 64), dtype=torch.float16, device=DEV) for _ in range(2)]
+    out = ops.append_paged_kv_cache_with_norm_rope(q[:, :0], k, v, *args, both[0], *tab)
+    assert out.shape == (len(t["pos"]), 0, 64)
+    ops.append_paged_kv_cache_with_norm_rope(q, k, v, *args, both[1], *tab)
+    assert torch.equal(both[0], both[1]) and both[0].any()
