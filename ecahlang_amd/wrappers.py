@@ -45,6 +45,12 @@ def _num_cus(device: torch.device) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
 
 
+@functools.lru_cache(maxsize=1024)
+def _fp8_workspace_bytes(*sizes: int) -> int:
+    """pkv_decode_fp8_workspace_bytes, a function of its arguments alone (1 us a call through ctypes)."""
+    return int(lib().pkv_decode_fp8_workspace_bytes(*sizes))
+
+
 def _unsupported(pos_encoding_mode, window_left, logits_soft_cap, rope_scale, rope_theta):
     if str(pos_encoding_mode).upper() != "NONE":
         raise NotImplementedError("pos_encoding_mode must be 'NONE' (RoPE is applied before the hook)")
@@ -222,10 +228,12 @@ class BatchDecodeWithPagedKVCacheWrapper:
         if self._ctas <= 0:
             raise ValueError("num_ctas must be positive")
         ws = self._workspace
+        if not (dev == ws.device == self._indices.device == self._last.device):
+            raise ValueError(f"the page table must be on the workspace's device, {ws.device}")
         pages = self._indices.numel()
-        need = lib().pkv_decode_fp8_workspace_bytes(self._batch, self._hq, self._hkv, self._d, self._ps, self._ctas, pages)
+        need = _fp8_workspace_bytes(self._batch, self._hq, self._hkv, self._d, self._ps, self._ctas, pages)
         if need < 0:
-            check(int(need), "decode plan")
+            check(need, "decode plan")
         if need > ws.numel() * ws.element_size():
             raise RuntimeError(f"decode workspace too small: need {need} bytes")
         counters = self._batch * self._hkv * -(-self._hq // self._hkv // 16)
@@ -255,8 +263,8 @@ class BatchDecodeWithPagedKVCacheWrapper:
         if hkv != self._hkv or d != self._d or ps != self._ps:
             raise ValueError("cache geometry differs from plan()")
         scales = scale_fields(kv_scales, pages, ps, hkv, cache_dt, dev)
-        if q.device != dev:
-            raise ValueError(f"q is on {q.device}, the cache on {dev}")
+        if q.device != dev or ws.device != dev:
+            raise ValueError(f"q is on {q.device}, the workspace on {ws.device}, the cache on {dev}")
         if out is None:
             out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dt, device=dev)
             st = out.stride()
