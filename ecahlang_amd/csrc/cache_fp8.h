@@ -175,7 +175,6 @@ inline bool head_dim_ok(int d) { return d > 0 && d <= 512 && d % 16 == 0; }
 // n / d = floor(n m / 2^(31+l)) (m is at most 2^32 - 1 but for d = 1, which keeps 2^31).
 struct Div {
   uint32_t m, l, d;
-  Div() = default;
   __host__ __device__ Div(uint32_t m_, uint32_t l_, uint32_t d_) : m(m_), l(l_), d(d_) {}
   explicit Div(uint32_t d_) : l(0), d(d_) {
     while ((1ull << l) < d) ++l;

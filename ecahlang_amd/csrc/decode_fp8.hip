@@ -60,7 +60,6 @@ template <> struct Codes<__hip_bfloat16> {
   static __device__ __forceinline__ uint32_t hi(uint32_t x) { return bitcast_<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.f, true)); }
 };
 
-
 // Parts whose weights the merge holds in the exchange buffer (16 columns of float2 each).
 __host__ __device__ constexpr int max_parts_of(int row, int waves) { return waves * (row / 16 - 1) * 8; }
 
@@ -400,7 +399,7 @@ __global__ __launch_bounds__(W * 64, HB * D == 256 ? 2 : 4) void decode_fp8_kern
     for (int c = 0; c < VW; ++c)  // dims VB (4 lg + i) + 4 c + (0 .. 3)
       s_o[wave][VW * i + c][lane] = f4{o[4 * c][i], o[4 * c + 1][i], o[4 * c + 2][i], o[4 * c + 3][i]} * cs;
   lds_barrier();
-    // (two heads a row: lanes lg / 2 hold the dims of head lg / 2)
+  // (two heads a row: lanes lg / 2 hold the dims of head lg / 2)
   if (lr < gc && (HB == 1 || lg / 2 == hn)) {
     const float inv = L > 0.f ? 1.f / L : 0.f;
     const int64_t hq = q0 + lr;
